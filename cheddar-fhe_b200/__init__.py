@@ -49,6 +49,7 @@ def lib():
         L.cfhe_prime.restype = C.c_uint32
         L.cfhe_galois_for_rotation.restype = C.c_uint32
         L.cfhe_kernel_launch_count.restype = C.c_ulonglong
+        L.cfhe_gemm_weight_bytes.restype = C.c_size_t
         _lib = L
     return _lib
 
@@ -283,13 +284,15 @@ class Engine:
             raise ValueError(kind)
         self._check(rc)
 
+    def gemm_weight_bytes(self, n_in, n_out, n_limbs):
+        return self.L.cfhe_gemm_weight_bytes(n_in, n_out, n_limbs)
+
     def gemm_pack_weights(self, weights, gidx):
         """weights: uint32 [n_limbs][n_in][n_out] in M-form; returns the packed device buffer."""
         w = np.ascontiguousarray(weights, dtype=np.uint32)
         n_limbs, n_in, n_out = w.shape
         g, gp = _ints(gidx)
-        self.L.cfhe_gemm_weight_bytes.restype = C.c_size_t
-        nbytes = self.L.cfhe_gemm_weight_bytes(n_in, n_out, n_limbs)
+        nbytes = self.gemm_weight_bytes(n_in, n_out, n_limbs)
         packed = self.torch.empty(nbytes, dtype=self.torch.uint8, device=f"cuda:{self.device}")
         self._check(self.L.cfhe_gemm_pack_weights(self.h, C.c_void_p(packed.data_ptr()),
                                                   w.ctypes.data_as(C.POINTER(C.c_uint32)), n_in, n_out, gp, len(g)))
@@ -298,6 +301,31 @@ class Engine:
     def ctpt_gemm_(self, ys, xs, packed, gidx):
         """ys[j] = sum_k W[k][j] * xs[k] on the tensor cores (cfhe_ctpt_gemm)."""
         self._check(self.K.ctpt_gemm(self.hp, ys, xs, packed, gidx))
+
+    # Operators of encrypted language models. Ciphertexts come as tensors whose last
+    # three dimensions are [2, limbs, N] (b, a) with any strides in front of a
+    # polynomial, or as lists (of lists) of such tensors.
+    def ctpt_project_(self, y, x, packed, gidx, bias=None, residual=None, res_scale=None):
+        """y[j] = sum_k W[k][j] * x[k] + (bias[:, j], 0) + res_scale * residual[j] on both
+        polynomials (cfhe_ctpt_project). y, residual: [n_out, 2, limbs, N], x: [n_in, 2,
+        limbs, N]; a list of residuals may hold None. bias: uint32 [limbs][n_out], res_scale:
+        uint32 [limbs] (None: 1), both M-form on the host. residual may be y."""
+        if packed.numel() < self.gemm_weight_bytes(len(x), len(y), len(gidx)):
+            raise ValueError("the packed weights are those of a smaller matrix")
+        self._check(self.K.ctpt_project(self.hp, self.device, y, x, packed, gidx, bias, residual, res_scale))
+
+    def rotary_(self, y, x, cos, sin, gidx, halves=False):
+        """Rotary positions (cfhe_rotary, cfhe_rotary_token): pairs of features (2i, 2i + 1),
+        or (i, i + dim / 2) with halves, of x [rows, dim, 2, limbs, N] turned by their angle
+        into y (which may be x). cos, sin: plaintexts [dim / 2, limbs, N], or uint32 words
+        [dim / 2][limbs] on the host where all slots are at one position."""
+        self._check(self.K.rotary(self.hp, self.device, y, x, cos, sin, gidx, halves))
+
+    def ctct_gemm_(self, d, left, right, gidx, decay=None):
+        """d[i][j] = decay[i][j] * sum_t left[i][t] (x) right[t][j] (cfhe_ctct_gemm), not
+        relinearised: d [m, n, 3, limbs, N], left [m, k, 2, limbs, N], right [k, n, 2, limbs,
+        N]; decay: plaintexts [m, n, limbs, N], uint32 words [m][n][limbs] on the host, or None."""
+        self._check(self.K.ctct_gemm(self.hp, self.device, d, left, right, gidx, decay))
 
     def sample_uniform_(self, dst, gidx, seed, stream=0):
         self._check(self.K.sample_uniform(self.hp, dst, gidx, seed, stream))

@@ -83,6 +83,42 @@ static int fill_limbs(const Context &c, NttArgs &a, const int *gidx,
   a.n_limbs = n_limbs;
   return 0;
 }
+// Host tables of a call on their way to the device: pointers first, then words.
+struct TableBlob {
+  std::vector<uint32_t> w;
+  template <typename T>
+  size_t pointers(T *const *p, size_t n) {  // null p: nothing; returns the byte offset
+    const size_t at = w.size() * sizeof(uint32_t);
+    if (!p) return at;
+    w.resize(w.size() + n * 2);
+    memcpy(reinterpret_cast<char *>(w.data()) + at, p, n * sizeof(void *));
+    return at;
+  }
+};
+// 1: every one of n pointers is there, on a 16-byte boundary if asked for
+template <typename T>
+static bool all_there(T *const *p, size_t n, bool aligned) {
+  if (!p) return false;
+  for (size_t i = 0; i < n; i++)
+    if (!p[i] || (aligned && (uintptr_t)p[i] % 16)) return false;
+  return true;
+}
+static int check_limbs(const Context &c, const int *gidx, int n_limbs) {
+  if (!gidx) return fail("null argument");
+  if (n_limbs < 1 || n_limbs > kMaxLimbs) return fail("between one and 64 limbs are expected");
+  for (int l = 0; l < n_limbs; l++)
+    if (gidx[l] < 0 || gidx[l] >= c.NP) return fail("prime index out of range");
+  return 0;
+}
+// An entry whose host tables may not find memory: no exception leaves it.
+template <typename F>
+static int guarded(F &&body) {
+  try {
+    return body();
+  } catch (const std::bad_alloc &) {
+    return fail("out of host memory");
+  }
+}
 }  // namespace cfhe
 
 using namespace cfhe;
@@ -800,6 +836,145 @@ int cfhe_ctpt_gemm(cfhe_context *h, uint32_t *const *y, const uint32_t *const *x
   CFHE_CUDA(cudaMemcpyAsync(dy, y, (size_t)n_out * sizeof(void *), cudaMemcpyHostToDevice, c.stream));
   CFHE_CUDA(cudaStreamSynchronize(c.stream));  // the host tables may go away after the call
   { int r_ = launch_ctpt_gemm(c, dy, dx, (const uint8_t *)packed, packed_x, n_in, n_out, gidx, n_limbs); c.mark("gemm"); return r_; }
+}
+
+int cfhe_ctpt_project(cfhe_context *h, uint32_t *const *yb, uint32_t *const *ya, const uint32_t *const *xb,
+                      const uint32_t *const *xa, const void *packed, int n_in, int n_out, const uint32_t *bias,
+                      const uint32_t *const *rb, const uint32_t *const *ra, const uint32_t *res_scale,
+                      const int *gidx, int n_limbs) {
+  CFHE_ENTER(h);
+  return guarded([&]() -> int {
+    Context &c = h->c;
+    if (n_in < 1 || n_in > 8192 || n_out < 1 || n_out > 8192) return fail("projection: 1 to 8192 inputs and outputs");
+    if (int r = check_limbs(c, gidx, n_limbs)) return r;
+    if ((uintptr_t)packed % 16) return fail("projection: packed weights on a 16-byte boundary are expected");
+    if (!packed || !all_there(xb, n_in, false) || !all_there(xa, n_in, false) || !all_there(yb, n_out, false) ||
+        !all_there(ya, n_out, false))
+      return fail("null argument");
+    if (!rb != !ra) return fail("projection: a residual needs both polynomials");
+    if (res_scale && !rb) return fail("projection: a residual scale without a residual");
+    for (int j = 0; rb && j < n_out; j++)
+      if (!rb[j] != !ra[j]) return fail("projection: a residual needs both polynomials");
+    const uint32_t *const *x[2] = {xb, xa}, *const *res[2] = {rb, ra};
+    uint32_t *const *y[2] = {yb, ya};
+    TableBlob blob;
+    size_t x_at[2], y_at[2], r_at[2];
+    for (int p = 0; p < 2; p++) {
+      x_at[p] = blob.pointers(x[p], n_in);
+      y_at[p] = blob.pointers(y[p], n_out);
+      r_at[p] = blob.pointers(res[p], n_out);
+    }
+    const size_t bias_at = blob.w.size() * sizeof(uint32_t);
+    if (bias)
+      for (int l = 0; l < n_limbs; l++)
+        for (int j = 0; j < n_out; j++) blob.w.push_back(bias[(size_t)l * n_out + j] % c.q[gidx[l]]);
+    uint32_t scale[kMaxLimbs];
+    for (int l = 0; l < n_limbs; l++) {
+      const uint32_t q = c.q[gidx[l]];
+      scale[l] = res_scale ? res_scale[l] % q : (uint32_t)((1ull << 32) % q);
+    }
+    const size_t limb = (gemm_scratch_bytes(n_in) + 255) / 256 * 256;
+    const size_t scratch = gemm_packs_ahead(n_out, n_limbs) ? 2 * limb : limb;
+    if (int r = ensure_workspace(c, scratch / 4 + blob.w.size())) return r;
+    char *base = reinterpret_cast<char *>(c.ws), *tab = base + scratch;
+    uint8_t *const packed_x[2] = {(uint8_t *)base, scratch > limb ? (uint8_t *)base + limb : nullptr};
+    if (int r = launch_upload(c, tab, blob.w.data(), blob.w.size())) return r;
+    for (int p = 0; p < 2; p++)
+      if (int r = launch_ctpt_project(c, (uint32_t *const *)(tab + y_at[p]), (const uint32_t *const *)(tab + x_at[p]),
+                                      (const uint8_t *)packed, packed_x, n_in, n_out,
+                                      bias && p == 0 ? (const uint32_t *)(tab + bias_at) : nullptr,
+                                      rb ? (const uint32_t *const *)(tab + r_at[p]) : nullptr, scale, gidx, n_limbs))
+        return r;
+    c.mark("gemm");
+    return 0;
+  });
+}
+
+static int rotary(Context &c, uint32_t *const *y, const uint32_t *const *x, int n_rows, int n_pairs, int halves,
+                  const uint32_t *const *cos, const uint32_t *const *sin, const uint32_t *cos_c,
+                  const uint32_t *sin_c, const int *gidx, int n_limbs) {
+  if (n_rows < 1 || n_pairs < 1 || (long long)n_rows * n_pairs > (1 << 20))
+    return fail("rotary positions: 1 to 2^20 pairs in all rows");
+  if (int r = check_limbs(c, gidx, n_limbs)) return r;
+  const size_t dim = 2 * (size_t)n_pairs, polys = n_rows * dim;
+  if (!all_there(x, polys, true) || !all_there(y, polys, true))
+    return fail("rotary positions: an operand is null or not on a 16-byte boundary");
+  std::vector<RotarySlot> slots((size_t)n_rows * n_pairs);
+  for (size_t r = 0, s = 0; r < (size_t)n_rows; r++)
+    for (size_t i = 0; i < (size_t)n_pairs; i++, s++) {
+      const size_t u = r * dim + (halves ? i : 2 * i), v = halves ? u + n_pairs : u + 1;
+      slots[s] = {x[u], x[v], y[u], y[v]};
+    }
+  const RotaryCall call = {n_rows, n_pairs, n_limbs, cos, sin, cos_c, sin_c, slots.data(), gidx};
+  { int r_ = launch_rotary(c, call); c.mark("elementwise"); return r_; }
+}
+
+int cfhe_rotary(cfhe_context *h, uint32_t *const *y, const uint32_t *const *x, int n_rows, int n_pairs, int halves,
+                const uint32_t *const *cos, const uint32_t *const *sin, const int *gidx, int n_limbs) {
+  CFHE_ENTER(h);
+  return guarded([&]() -> int {
+    if (n_pairs > 0 && (!all_there(cos, n_pairs, true) || !all_there(sin, n_pairs, true)))
+      return fail("rotary positions: a plaintext is null or not on a 16-byte boundary");
+    return rotary(h->c, y, x, n_rows, n_pairs, halves, cos, sin, nullptr, nullptr, gidx, n_limbs);
+  });
+}
+
+int cfhe_rotary_token(cfhe_context *h, uint32_t *const *y, const uint32_t *const *x, int n_rows, int n_pairs,
+                      int halves, const uint32_t *cos, const uint32_t *sin, const int *gidx, int n_limbs) {
+  CFHE_ENTER(h);
+  return guarded([&]() -> int {
+    if (!cos || !sin) return fail("null argument");
+    return rotary(h->c, y, x, n_rows, n_pairs, halves, nullptr, nullptr, cos, sin, gidx, n_limbs);
+  });
+}
+
+int cfhe_ctct_gemm(cfhe_context *h, uint32_t *const *d0, uint32_t *const *d1, uint32_t *const *d2,
+                   const uint32_t *const *lb, const uint32_t *const *la, const uint32_t *const *rb,
+                   const uint32_t *const *ra, int m, int k, int n, const uint32_t *const *decay_pt,
+                   const uint32_t *decay_const, const int *gidx, int n_limbs) {
+  CFHE_ENTER(h);
+  return guarded([&]() -> int {
+    Context &c = h->c;
+    if (m < 1 || m > 8192 || k < 1 || k > 8192 || n < 1 || n > 8192 || (long long)m * n > 65535 ||
+        (long long)m * k + (long long)k * n > (1 << 20))
+      return fail("ct-ct GEMM: unsupported shape");
+    if (int r = check_limbs(c, gidx, n_limbs)) return r;
+    if (decay_pt && decay_const) return fail("ct-ct GEMM: plaintext or constant decay, not both");
+    const size_t mk = (size_t)m * k, kn = (size_t)k * n, mn = (size_t)m * n;
+    if (!all_there(lb, mk, true) || !all_there(la, mk, true) || !all_there(rb, kn, true) || !all_there(ra, kn, true) ||
+        !all_there(d0, mn, true) || !all_there(d1, mn, true) || !all_there(d2, mn, true) ||
+        (decay_pt && !all_there(decay_pt, mn, true)))
+      return fail("ct-ct GEMM: an operand is null or not on a 16-byte boundary");
+    TableBlob blob;
+    blob.w.reserve(2 * (2 * (mk + kn) + 4 * mn) + (decay_const ? mn * n_limbs : 0));
+    blob.pointers(lb, mk);
+    blob.pointers(la, mk);
+    blob.pointers(rb, kn);
+    blob.pointers(ra, kn);
+    blob.pointers(d0, mn);
+    blob.pointers(d1, mn);
+    blob.pointers(d2, mn);
+    blob.pointers(decay_pt, mn);
+    const size_t consts_at = blob.w.size();
+    if (decay_const)
+      for (size_t o = 0; o < mn; o++)
+        for (int l = 0; l < n_limbs; l++) blob.w.push_back(decay_const[o * n_limbs + l] % c.q[gidx[l]]);
+    if (int r = ensure_workspace(c, blob.w.size())) return r;
+    if (int r = launch_upload(c, c.ws, blob.w.data(), blob.w.size())) return r;
+    CtctArgs a;
+    a.m = m;
+    a.k = k;
+    a.n = n;
+    a.n_limbs = n_limbs;
+    a.table = reinterpret_cast<const uint32_t *const *>(c.ws);
+    a.consts = decay_const ? c.ws + consts_at : nullptr;
+    a.weights = decay_pt != nullptr;
+    for (int l = 0; l < n_limbs; l++) {
+      a.q[l] = c.q[gidx[l]];
+      a.nqinv[l] = c.nqinv[gidx[l]];
+    }
+    { int r_ = launch_ctct_gemm(c, a); c.mark("elementwise"); return r_; }
+  });
 }
 
 int cfhe_sample_uniform(cfhe_context *h, uint32_t *dst, const int *gidx, int n_limbs,

@@ -74,6 +74,11 @@ struct GemmArgs {
   const uint32_t *const *x;
   size_t next_off;
   int n_in;
+  // projection (EPI): what joins an output word before it is stored; null where
+  // there is none. A residual's table holds a null for an output without one.
+  const uint32_t *const *res;  // n_out residual polynomials, multiplied by res_scale (M-form)
+  const uint32_t *bias;        // n_out words of this limb
+  uint32_t res_scale;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -146,6 +151,7 @@ __device__ __forceinline__ void store_chunk(uint8_t *xp, int k_chunks, int m_til
   *reinterpret_cast<uint4 *>(xp + ((size_t)m_tile * k_chunks + t) * (kGmTile * 16) + row * 16) = w;
 }
 
+template <bool EPI>
 __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_constant__ GemmArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *sA = smem;                               // [stage][4][16][8][16]
@@ -263,9 +269,17 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
           const int j = n_tile * kGmOutTile + j0 + e;
           if (j < a.n_out) {
             // V = d0 + d1 2^8 + d2 2^16 + d3 2^24, every d below 2^31
-            const uint64_t v = (uint64_t)d[4 * e] + ((uint64_t)d[4 * e + 1] << 8) +
-                               ((uint64_t)d[4 * e + 2] << 16) + ((uint64_t)d[4 * e + 3] << 24);
-            a.y[j][col] = mont_reduce(v, q, nq);
+            uint64_t v = (uint64_t)d[4 * e] + ((uint64_t)d[4 * e + 1] << 8) +
+                         ((uint64_t)d[4 * e + 2] << 16) + ((uint64_t)d[4 * e + 3] << 24);
+            if constexpr (EPI) {
+              // v < 2^23 q and the product below q 2^31: still one reduction
+              const uint32_t *r = a.res ? a.res[j] : nullptr;
+              if (r) v += (uint64_t)r[col] * a.res_scale;
+              const uint32_t y = mont_reduce(v, q, nq);
+              a.y[j][col] = a.bias ? add_mod(y, a.bias[j], q) : y;
+            } else {
+              a.y[j][col] = mont_reduce(v, q, nq);
+            }
           }
         }
       }
@@ -340,11 +354,13 @@ bool gemm_packs_ahead(int n_out, int n_limbs) {
   return n_limbs > 1 && (n_out + kGmOutTile - 1) / kGmOutTile >= 3;
 }
 
-int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
-                     uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs) {
+template <bool EPI>
+static int launch_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
+                       uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs,
+                       const uint32_t *const *res, const uint32_t *bias, const uint32_t *res_scale) {
   static PerDeviceOnce once;
   if (int r = once.run(c.device, [] {
-        CFHE_CUDA(cudaFuncSetAttribute(gemm_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem));
+        CFHE_CUDA(cudaFuncSetAttribute(gemm_tc_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem));
         return 0;
       }))
     return r;
@@ -380,11 +396,28 @@ int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const
     a.q = c.q[gidx[l]];
     a.nqinv = c.nqinv[gidx[l]];
     a.error_flag = c.d_error_flag;
-    CFHE_CUDA(launch_kernel(c.use_pdl, gemm_tc_kernel, dim3(n_tiles, kN / kGmTile), dim3(kGmThreads), kGmSmem,
+    a.res = res;
+    a.bias = bias ? bias + (size_t)l * n_out : nullptr;
+    a.res_scale = res_scale ? res_scale[l] : 0;
+    CFHE_CUDA(launch_kernel(c.use_pdl, gemm_tc_kernel<EPI>, dim3(n_tiles, kN / kGmTile), dim3(kGmThreads), kGmSmem,
                             c.stream, a));
   }
   CFHE_CUDA(cudaGetLastError());
   return 0;
+}
+
+int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
+                     uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs) {
+  return launch_gemm<false>(c, y, x, wp, scratch, n_in, n_out, gidx, n_limbs, nullptr, nullptr, nullptr);
+}
+
+// One polynomial of a projection: res a device table of n_out pointers (null
+// entries: no residual) or null, bias [n_limbs][n_out] on the device or null,
+// res_scale [n_limbs] on the host.
+int launch_ctpt_project(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
+                        uint8_t *const *scratch, int n_in, int n_out, const uint32_t *bias,
+                        const uint32_t *const *res, const uint32_t *res_scale, const int *gidx, int n_limbs) {
+  return launch_gemm<true>(c, y, x, wp, scratch, n_in, n_out, gidx, n_limbs, res, bias, res_scale);
 }
 
 }  // namespace cfhe

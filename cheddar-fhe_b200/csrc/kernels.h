@@ -174,6 +174,39 @@ bool gemm_packs_ahead(int n_out, int n_limbs);
 void gemm_pack_weights_limb(uint8_t *out, const uint32_t *w, int n_in, int n_out, uint32_t q);
 int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
                      uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs);
+int launch_ctpt_project(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
+                        uint8_t *const *scratch, int n_in, int n_out, const uint32_t *bias,
+                        const uint32_t *const *res, const uint32_t *res_scale, const int *gidx, int n_limbs);
+// upload.cu: `words` host words to the device through kernel parameters
+int launch_upload(const Context &c, void *dst, const void *src, size_t words);
+
+// rotary.cu: (u, v) -> (cos u - sin v, sin u + cos v) on pairs of polynomials;
+// operands of pair i in row r at [r * n_pairs + i]. cos, sin: n_pairs device
+// polynomials each, or (cos_c, sin_c) words [n_pairs][n_limbs] on the host.
+struct RotarySlot {
+  const uint32_t *u, *v;
+  uint32_t *yu, *yv;
+};
+struct RotaryCall {
+  int n_rows, n_pairs, n_limbs;
+  const uint32_t *const *cos, *const *sin;
+  const uint32_t *cos_c, *sin_c;
+  const RotarySlot *slots;
+  const int *gidx;
+};
+int launch_rotary(const Context &ctx, const RotaryCall &call);
+
+// ctct_gemm.cu: D[i][j] = w[i][j] (*) sum_t L[i][t] (x) R[t][j], three parts
+struct CtctArgs {
+  int m, k, n, n_limbs;
+  // device table: left b [m*k], left a, right b [k*n], right a, d0 [m*n], d1, d2,
+  // then weight plaintexts [m*n] where weights is 1
+  const uint32_t *const *table;
+  const uint32_t *consts;  // device, [m*n][n_limbs], or null
+  int weights;             // plaintext weights present
+  uint32_t q[kMaxLimbs], nqinv[kMaxLimbs];
+};
+int launch_ctct_gemm(const Context &ctx, const CtctArgs &args);
 // sampling.cu: client-side sampling and encryption
 constexpr int kErrorCdfEntries = 97;
 void error_cdf_table(double sigma, uint64_t *cdf);

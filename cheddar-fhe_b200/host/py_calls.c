@@ -14,7 +14,14 @@
 
 #include "../../include/cheddar_b200.h"
 
-static PyObject *s_data_ptr, *s_dim, *s_size, *s_stride;
+/* entry points that a library built before them does not have: the module loads
+ * beside such a library too, and only their calls are errors then */
+#pragma weak cfhe_ctpt_project
+#pragma weak cfhe_rotary
+#pragma weak cfhe_rotary_token
+#pragma weak cfhe_ctct_gemm
+
+static PyObject *s_data_ptr, *s_dim, *s_size, *s_stride, *s_shape, *s_element_size, *s_get_device;
 static PyObject *as_int32, *as_uint32; /* converters for arguments that are no ready-made 32-bit array */
 static PyObject *zero;
 
@@ -190,6 +197,133 @@ static int get_shape(PyObject *t, long long *polys, long long *stride) {
   return 0;
 }
 
+/* ---- matrices of ciphertexts or plaintexts: one tensor [rows(, cols)(, parts), limbs, N]
+ * with any strides in front of the words, or a list (of lists) of the tensors inside ---- */
+typedef struct {
+  void **p; /* [part][rows * cols], one part for plaintexts */
+  Py_ssize_t rows, cols;
+} ct_table;
+
+typedef struct {
+  long long device, limbs, n;
+} ct_shape;
+
+static void free_cts(ct_table *t) {
+  PyMem_Free(t->p);
+  t->p = NULL;
+}
+
+static int new_cts(ct_table *t, Py_ssize_t rows, Py_ssize_t cols, int parts) {
+  t->rows = rows;
+  t->cols = cols;
+  t->p = (void **)PyMem_Calloc((size_t)(rows * cols * (parts ? parts : 1)) + 1, sizeof(void *));
+  if (!t->p) PyErr_NoMemory();
+  return t->p ? 0 : -1;
+}
+
+/* dimensions and strides of a tensor of 32-bit words on the engine's device
+ * with `lead` leading dimensions, a dimension of `parts` (if any), limbs and words */
+static int get_layout(PyObject *o, int lead, int parts, const ct_shape *want, char **base, long long *dim,
+                      long long *stride) {
+  const int nd = lead + (parts ? 1 : 0) + 2;
+  int ok = 0;
+  long long v;
+  PyObject *shape = NULL, *st = NULL, *e = PyObject_CallMethodNoArgs(o, s_element_size);
+  if (!e || get_ll(e, &v)) goto done;
+  if (v != 4) {
+    PyErr_SetString(PyExc_ValueError, "tensors of 32-bit words are expected");
+    goto done;
+  }
+  Py_DECREF(e);
+  e = PyObject_CallMethodNoArgs(o, s_get_device);
+  if (!e || get_ll(e, &v)) goto done;
+  if (v != want->device) {
+    PyErr_SetString(PyExc_ValueError, "a tensor is not on the engine's device");
+    goto done;
+  }
+  shape = PyObject_GetAttr(o, s_shape);
+  st = shape ? PyObject_CallMethodNoArgs(o, s_stride) : NULL;
+  if (!st) goto done;
+  if (!PyTuple_Check(shape) || !PyTuple_Check(st) || PyTuple_GET_SIZE(shape) != nd || PyTuple_GET_SIZE(st) != nd) {
+    PyErr_Format(PyExc_ValueError, "a tensor of %d dimensions is expected", nd);
+    goto done;
+  }
+  for (int i = 0; i < nd; i++)
+    if (get_ll(PyTuple_GET_ITEM(shape, i), dim + i) || get_ll(PyTuple_GET_ITEM(st, i), stride + i)) goto done;
+  if (dim[nd - 1] != want->n || dim[nd - 2] != want->limbs || (parts && dim[lead] != parts)) {
+    PyErr_SetString(PyExc_ValueError, "a tensor has another number of polynomials, limbs or words than the call");
+    goto done;
+  }
+  if (stride[nd - 1] != 1 || (want->limbs > 1 && stride[nd - 2] != want->n)) {
+    PyErr_SetString(PyExc_ValueError, "the limbs of a polynomial have to lie one after the other");
+    goto done;
+  }
+  ok = get_ptr(o, (void **)base) == 0;
+done:
+  Py_XDECREF(e);
+  Py_XDECREF(shape);
+  Py_XDECREF(st);
+  return ok ? 0 : -1;
+}
+
+/* lead: 1 (a list of ciphertexts) or 2 (a matrix); holes: a list may hold None */
+static int get_cts(PyObject *o, int lead, int parts, int holes, const ct_shape *want, ct_table *t) {
+  long long dim[5], stride[5];
+  char *base;
+  t->p = NULL;
+  const int each = parts ? parts : 1;
+  if (!PyList_Check(o) && !PyTuple_Check(o)) {
+    if (get_layout(o, lead, parts, want, &base, dim, stride)) return -1;
+    const long long cols = lead == 2 ? dim[1] : 1, cs = lead == 2 ? stride[1] : 0;
+    if (new_cts(t, dim[0], cols, parts)) return -1;
+    for (int p = 0; p < each; p++)
+      for (long long r = 0; r < dim[0]; r++)
+        for (long long c = 0; c < cols; c++)
+          t->p[(p * dim[0] + r) * cols + c] = base + 4 * (r * stride[0] + c * cs + (parts ? p * stride[lead] : 0));
+    return 0;
+  }
+  const Py_ssize_t rows = PySequence_Fast_GET_SIZE(o);
+  Py_ssize_t cols = 1;
+  if (lead == 2 && rows) {
+    PyObject *first = PySequence_Fast_GET_ITEM(o, 0);
+    if (!PyList_Check(first) && !PyTuple_Check(first)) {
+      PyErr_SetString(PyExc_TypeError, "a tensor or a list of rows is expected");
+      return -1;
+    }
+    cols = PySequence_Fast_GET_SIZE(first);
+  }
+  if (new_cts(t, rows, cols, parts)) return -1;
+  for (Py_ssize_t r = 0; r < rows; r++) {
+    PyObject *row = PySequence_Fast_GET_ITEM(o, r);
+    if (lead == 2 && ((!PyList_Check(row) && !PyTuple_Check(row)) || PySequence_Fast_GET_SIZE(row) != cols)) {
+      PyErr_SetString(PyExc_ValueError, "the rows of a matrix have to be lists of one length");
+      free_cts(t);
+      return -1;
+    }
+    for (Py_ssize_t c = 0; c < cols; c++) {
+      PyObject *x = lead == 2 ? PySequence_Fast_GET_ITEM(row, c) : row;
+      if (holes && x == Py_None) continue;
+      if (get_layout(x, 0, parts, want, &base, dim, stride)) {
+        free_cts(t);
+        return -1;
+      }
+      for (int p = 0; p < each; p++) t->p[(p * rows + r) * cols + c] = base + (parts ? 4 * p * stride[0] : 0);
+    }
+  }
+  return 0;
+}
+
+/* host words; None: none. Any other count than `count` is an error. */
+static int get_words(PyObject *o, long long count, int_list *l) {
+  if (get_constants(o, l)) return -1;
+  if (o != Py_None && l->b.len != 4 * count) {
+    PyErr_SetString(PyExc_ValueError, "wrong number of constants");
+    free_ints(l);
+    return -1;
+  }
+  return 0;
+}
+
 #define HANDLE(o) ((cfhe_context *)PyLong_AsVoidPtr(o))
 #define NEED(count)                                                     \
   if (n != (count)) {                                                   \
@@ -200,6 +334,11 @@ static int get_shape(PyObject *t, long long *polys, long long *stride) {
   Py_BEGIN_ALLOW_THREADS;  \
   rc = (call);             \
   Py_END_ALLOW_THREADS
+#define HAVE(entry)                                                          \
+  if (!entry) {                                                              \
+    PyErr_SetString(PyExc_RuntimeError, "the library does not have " #entry); \
+    return NULL;                                                             \
+  }
 typedef uint32_t u32;
 
 /* ---- transforms: (handle, dst, src, gidx, mont_conv) ---- */
@@ -582,6 +721,136 @@ free_y:
   return ret;
 }
 
+/* (handle, device, y, x, packed, gidx, bias, residual, res_scale): y, x and residual
+ * lists of ciphertexts; residual (whose list may hold None), bias and res_scale may be None */
+static PyObject *py_ctpt_project(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+  NEED(9)
+  HAVE(cfhe_ctpt_project)
+  ct_table y = {0}, x = {0}, r = {0};
+  int_list g = {0}, bias = {0}, scale = {0};
+  ct_shape want;
+  void *w;
+  int rc;
+  PyObject *ret = NULL;
+  if (get_ll(a[1], &want.device) || get_ptr(a[4], &w) || get_ints(a[5], 'i', &g)) return NULL;
+  want.limbs = g.n;
+  want.n = cfhe_degree(HANDLE(a[0]));
+  if (get_cts(a[2], 1, 2, 0, &want, &y) || get_cts(a[3], 1, 2, 0, &want, &x)) goto done;
+  if (a[7] != Py_None) {
+    if (get_cts(a[7], 1, 2, 1, &want, &r)) goto done;
+    if (r.rows != y.rows) {
+      PyErr_SetString(PyExc_ValueError, "one residual per output is expected");
+      goto done;
+    }
+  }
+  if (get_words(a[6], want.limbs * y.rows, &bias) || get_words(a[8], want.limbs, &scale)) goto done;
+  ENTER(cfhe_ctpt_project(HANDLE(a[0]), (u32 *const *)y.p, (u32 *const *)y.p + y.rows, (const u32 *const *)x.p,
+                          (const u32 *const *)x.p + x.rows, w, (int)x.rows, (int)y.rows, bias.p,
+                          (const u32 *const *)r.p, r.p ? (const u32 *const *)r.p + r.rows : NULL, scale.p, g.p, g.n));
+  ret = PyLong_FromLong(rc);
+done:
+  free_cts(&y);
+  free_cts(&x);
+  free_cts(&r);
+  free_ints(&bias);
+  free_ints(&scale);
+  free_ints(&g);
+  return ret;
+}
+
+/* (handle, device, y, x, cos, sin, gidx, halves): y, x matrices of ciphertexts; cos and sin
+ * lists of plaintexts, or arrays of words [pairs][limbs] */
+static PyObject *py_rotary(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+  NEED(8)
+  HAVE(cfhe_rotary)
+  HAVE(cfhe_rotary_token)
+  ct_table y = {0}, x = {0}, c = {0}, s = {0};
+  int_list g = {0}, cw = {0}, sw = {0};
+  ct_shape want;
+  long long halves;
+  int rc;
+  PyObject *ret = NULL;
+  if (get_ll(a[1], &want.device) || get_converted(a[7], &halves) || get_ints(a[6], 'i', &g)) return NULL;
+  want.limbs = g.n;
+  want.n = cfhe_degree(HANDLE(a[0]));
+  if (get_cts(a[2], 2, 2, 0, &want, &y) || get_cts(a[3], 2, 2, 0, &want, &x)) goto done;
+  if (y.rows != x.rows || y.cols != x.cols || x.cols % 2) {
+    PyErr_SetString(PyExc_ValueError, "inputs and outputs of the same even number of features are expected");
+    goto done;
+  }
+  const Py_ssize_t pairs = x.cols / 2;
+  u32 *const *yp = (u32 *const *)y.p;
+  const u32 *const *xp = (const u32 *const *)x.p;
+  if (PyObject_CheckBuffer(a[4])) {
+    if (get_words(a[4], pairs * want.limbs, &cw) || get_words(a[5], pairs * want.limbs, &sw)) goto done;
+    ENTER(cfhe_rotary_token(HANDLE(a[0]), yp, xp, (int)(2 * x.rows), (int)pairs, halves != 0, cw.p, sw.p, g.p, g.n));
+  } else {
+    if (get_cts(a[4], 1, 0, 0, &want, &c) || get_cts(a[5], 1, 0, 0, &want, &s)) goto done;
+    if (c.rows != pairs || s.rows != pairs) {
+      PyErr_SetString(PyExc_ValueError, "one cosine and one sine per pair of features are expected");
+      goto done;
+    }
+    ENTER(cfhe_rotary(HANDLE(a[0]), yp, xp, (int)(2 * x.rows), (int)pairs, halves != 0, (const u32 *const *)c.p,
+                      (const u32 *const *)s.p, g.p, g.n));
+  }
+  ret = PyLong_FromLong(rc);
+done:
+  free_cts(&y);
+  free_cts(&x);
+  free_cts(&c);
+  free_cts(&s);
+  free_ints(&cw);
+  free_ints(&sw);
+  free_ints(&g);
+  return ret;
+}
+
+/* (handle, device, d, left, right, gidx, decay): matrices of three-part products, of
+ * ciphertexts and of ciphertexts; decay None, a matrix of plaintexts or words [m][n][limbs] */
+static PyObject *py_ctct_gemm(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+  NEED(7)
+  HAVE(cfhe_ctct_gemm)
+  ct_table d = {0}, l = {0}, r = {0}, w = {0};
+  int_list g = {0}, ww = {0};
+  ct_shape want;
+  int rc;
+  PyObject *ret = NULL;
+  if (get_ll(a[1], &want.device) || get_ints(a[5], 'i', &g)) return NULL;
+  want.limbs = g.n;
+  want.n = cfhe_degree(HANDLE(a[0]));
+  if (get_cts(a[2], 2, 3, 0, &want, &d) || get_cts(a[3], 2, 2, 0, &want, &l) || get_cts(a[4], 2, 2, 0, &want, &r))
+    goto done;
+  if (l.rows != d.rows || r.cols != d.cols || l.cols != r.rows) {
+    PyErr_SetString(PyExc_ValueError, "the sizes of the matrices do not fit");
+    goto done;
+  }
+  const Py_ssize_t mn = d.rows * d.cols, mk = l.rows * l.cols, kn = r.rows * r.cols;
+  if (a[6] != Py_None) {
+    if (PyObject_CheckBuffer(a[6])) {
+      if (get_words(a[6], mn * want.limbs, &ww)) goto done;
+    } else {
+      if (get_cts(a[6], 2, 0, 0, &want, &w)) goto done;
+      if (w.rows != d.rows || w.cols != d.cols) {
+        PyErr_SetString(PyExc_ValueError, "one decay per result is expected");
+        goto done;
+      }
+    }
+  }
+  u32 *const *dp = (u32 *const *)d.p;
+  const u32 *const *lp = (const u32 *const *)l.p, *const *rp = (const u32 *const *)r.p;
+  ENTER(cfhe_ctct_gemm(HANDLE(a[0]), dp, dp + mn, dp + 2 * mn, lp, lp + mk, rp, rp + kn, (int)d.rows, (int)l.cols,
+                       (int)d.cols, (const u32 *const *)w.p, ww.p, g.p, g.n));
+  ret = PyLong_FromLong(rc);
+done:
+  free_cts(&d);
+  free_cts(&l);
+  free_cts(&r);
+  free_cts(&w);
+  free_ints(&ww);
+  free_ints(&g);
+  return ret;
+}
+
 /* ---- client side: (handle, dst, gidx, seed, stream) ---- */
 static PyObject *py_sample_uniform(PyObject *self, PyObject *const *a, Py_ssize_t n) {
   NEED(5)
@@ -665,7 +934,7 @@ static PyObject *py_set_converters(PyObject *self, PyObject *const *a, Py_ssize_
 static PyMethodDef methods[] = {M(ntt),           M(intt),      M(binary),        M(const_op),
                                 M(elementwise_multi), M(tensor), M(permute),      M(moddown),
                                 M(keyswitch),     M(hmult),     M(hoisted_rotations), M(linear_transform),
-                                M(ctpt_gemm),     M(sample_uniform), M(sample_error), M(encrypt),
+                                M(ctpt_gemm),     M(ctpt_project), M(rotary), M(ctct_gemm), M(sample_uniform), M(sample_error), M(encrypt),
                                 M(encode_coeffs),
                                 M(set_converters), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "cheddar_b200_calls", NULL, -1, methods,
@@ -677,6 +946,10 @@ PyMODINIT_FUNC PyInit_cheddar_b200_calls(void) {
   s_size = PyUnicode_InternFromString("size");
   s_stride = PyUnicode_InternFromString("stride");
   zero = PyLong_FromLong(0);
-  if (!s_data_ptr || !s_dim || !s_size || !s_stride || !zero) return NULL;
+  s_shape = PyUnicode_InternFromString("shape");
+  s_element_size = PyUnicode_InternFromString("element_size");
+  s_get_device = PyUnicode_InternFromString("get_device");
+  if (!s_data_ptr || !s_dim || !s_size || !s_stride || !zero || !s_shape || !s_element_size || !s_get_device)
+    return NULL;
   return PyModule_Create(&module);
 }

@@ -215,6 +215,62 @@ CFHE_API int cfhe_gemm_pack_weights(cfhe_context *ctx, void *packed, const uint3
                                     int n_out, const int *gidx, int n_limbs);
 CFHE_API int cfhe_ctpt_gemm(cfhe_context *ctx, uint32_t *const *y, const uint32_t *const *x,
                             const void *packed, int n_in, int n_out, const int *gidx, int n_limbs);
+/* Projection of ciphertexts with its epilogue, one call for both polynomials:
+ *   (yb, ya)[j] = sum_k W[l][k][j] * (xb, xa)[k] + (bias[l][j], 0)
+ *                 + res_scale[l] * (rb, ra)[j]
+ * on every listed limb l, the product on the tensor cores as in cfhe_ctpt_gemm
+ * (packed from cfhe_gemm_pack_weights). The sum is formed before a rescale, so
+ * bias and residual come at the scale of the product: a constant's word per limb
+ * (M-form), a ciphertext at the level of x times a constant (M-form) that brings
+ * it there.
+ *   bias       HOST [n_limbs][n_out], or NULL
+ *   rb, ra     HOST arrays of n_out DEVICE pointers, both NULL without residual;
+ *              an output without one holds NULL in both
+ *   res_scale  HOST [n_limbs], or NULL for the factor 1
+ * n_in and n_out up to 8192. A residual may be its own output; apart from that
+ * no output may overlap an input. Same words as cfhe_ctpt_gemm on either
+ * polynomial, cfhe_const_op (multiply and add, add) on the result. No function
+ * of the outputs is applied: on encrypted values a non-linear one is a product
+ * of ciphertexts. */
+CFHE_API int cfhe_ctpt_project(cfhe_context *ctx, uint32_t *const *yb, uint32_t *const *ya,
+                               const uint32_t *const *xb, const uint32_t *const *xa, const void *packed,
+                               int n_in, int n_out, const uint32_t *bias, const uint32_t *const *rb,
+                               const uint32_t *const *ra, const uint32_t *res_scale, const int *gidx,
+                               int n_limbs);
+/* Rotary positions: pairs of features turned by the angle of their token's
+ * position,  (u, v) -> (cos u - sin v, sin u + cos v)  on every listed limb.
+ * x, y: HOST arrays of n_rows * 2 n_pairs DEVICE pointers, a row being one
+ * polynomial (b or a) of the features of one head of the queries or keys; pair i
+ * of a row is (2i, 2i + 1), or (i, i + n_pairs) where halves is not 0. y may be
+ * x; no other overlap.
+ *   cfhe_rotary        cos, sin: HOST arrays of n_pairs DEVICE pointers to
+ *                      plaintexts (each slot holds its own token's value)
+ *   cfhe_rotary_token  cos, sin: HOST words [n_pairs][n_limbs] in M-form (every
+ *                      slot at the same position: one new token)
+ * Positions on several axes are in the angles: pair i follows the axis that its
+ * cos and sin were made for. All polynomials on 16-byte boundaries. Same words as
+ * cfhe_paccum / cfhe_caccum of two terms (with q - sin for the first). */
+CFHE_API int cfhe_rotary(cfhe_context *ctx, uint32_t *const *y, const uint32_t *const *x, int n_rows,
+                         int n_pairs, int halves, const uint32_t *const *cos, const uint32_t *const *sin,
+                         const int *gidx, int n_limbs);
+CFHE_API int cfhe_rotary_token(cfhe_context *ctx, uint32_t *const *y, const uint32_t *const *x, int n_rows,
+                               int n_pairs, int halves, const uint32_t *cos, const uint32_t *sin,
+                               const int *gidx, int n_limbs);
+/* Matrix product of ciphertexts with three-part results (not relinearised):
+ *   (d0, d1, d2)[i][j] = w[i][j] (*) sum_t (lb, la)[i][t] (x) (rb, ra)[t][j]
+ * for m x k left and k x n right ciphertexts, all tables HOST arrays of DEVICE
+ * pointers, row after row: the scores and the weighted values of attention over
+ * encrypted tokens. w, the decay (and mask) of linear attention:
+ *   decay_pt     HOST array of m n DEVICE pointers to plaintexts, or NULL
+ *   decay_const  HOST words [m * n][n_limbs] in M-form, or NULL
+ * at most one of the two. m, k, n from 1 to 8192, at most 65535 results and 2^20
+ * operands; outputs overlap nothing; polynomials on 16-byte boundaries. Same
+ * words as cfhe_tensor_accum per result, then cfhe_binary / cfhe_const_op
+ * (multiply) on its three parts. */
+CFHE_API int cfhe_ctct_gemm(cfhe_context *ctx, uint32_t *const *d0, uint32_t *const *d1, uint32_t *const *d2,
+                            const uint32_t *const *lb, const uint32_t *const *la, const uint32_t *const *rb,
+                            const uint32_t *const *ra, int m, int k, int n, const uint32_t *const *decay_pt,
+                            const uint32_t *decay_const, const int *gidx, int n_limbs);
 /* Client-side sampling and encryption on the device (the reference samples on
  * the host and uploads: src/UserInterface.cu:223-276, 366-458; Random,
  * include/Random.h). Words are a pure function of (seed, stream, prime index,
