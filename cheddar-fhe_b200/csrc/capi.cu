@@ -945,34 +945,40 @@ int cfhe_ctct_gemm(cfhe_context *h, uint32_t *const *d0, uint32_t *const *d1, ui
         !all_there(d0, mn, true) || !all_there(d1, mn, true) || !all_there(d2, mn, true) ||
         (decay_pt && !all_there(decay_pt, mn, true)))
       return fail("ct-ct GEMM: an operand is null or not on a 16-byte boundary");
-    TableBlob blob;
-    blob.w.reserve(2 * (2 * (mk + kn) + 4 * mn) + (decay_const ? mn * n_limbs : 0));
-    blob.pointers(lb, mk);
-    blob.pointers(la, mk);
-    blob.pointers(rb, kn);
-    blob.pointers(ra, kn);
-    blob.pointers(d0, mn);
-    blob.pointers(d1, mn);
-    blob.pointers(d2, mn);
-    blob.pointers(decay_pt, mn);
-    const size_t consts_at = blob.w.size();
-    if (decay_const)
-      for (size_t o = 0; o < mn; o++)
-        for (int l = 0; l < n_limbs; l++) blob.w.push_back(decay_const[o * n_limbs + l] % c.q[gidx[l]]);
-    if (int r = ensure_workspace(c, blob.w.size())) return r;
-    if (int r = launch_upload(c, c.ws, blob.w.data(), blob.w.size())) return r;
+    // the product of the transposes where there are more rows than columns
+    const bool turned = m > n;
     CtctArgs a;
-    a.m = m;
+    a.m = turned ? n : m;
+    a.n = turned ? m : n;
     a.k = k;
-    a.n = n;
     a.n_limbs = n_limbs;
-    a.table = reinterpret_cast<const uint32_t *const *>(c.ws);
-    a.consts = decay_const ? c.ws + consts_at : nullptr;
-    a.weights = decay_pt != nullptr;
     for (int l = 0; l < n_limbs; l++) {
       a.q[l] = c.q[gidx[l]];
       a.nqinv[l] = c.nqinv[gidx[l]];
     }
+    const size_t out_at = (mk + kn) * sizeof(CtctPair), consts_at = out_at + mn * sizeof(CtctOut);
+    std::vector<char> blob(consts_at + (decay_const ? mn * n_limbs * sizeof(uint32_t) : 0));
+    CtctPair *const p0 = reinterpret_cast<CtctPair *>(blob.data()), *const p1 = p0 + (size_t)a.m * k;
+    CtctPair *const left = turned ? p1 : p0, *const right = turned ? p0 : p1;
+    CtctOut *const out = reinterpret_cast<CtctOut *>(blob.data() + out_at);
+    uint32_t *const consts = reinterpret_cast<uint32_t *>(blob.data() + consts_at);
+    for (int i = 0; i < m; i++)
+      for (int t = 0; t < k; t++) left[(size_t)t * m + i] = {lb[(size_t)i * k + t], la[(size_t)i * k + t]};
+    for (size_t e = 0; e < kn; e++) right[e] = {rb[e], ra[e]};
+    for (int i = 0; i < m; i++)
+      for (int j = 0; j < n; j++) {
+        const size_t from = (size_t)i * n + j, to = turned ? (size_t)j * m + i : from;
+        out[to] = {d0[from], d1[from], d2[from], decay_pt ? decay_pt[from] : nullptr};
+        for (int l = 0; decay_const && l < n_limbs; l++)
+          consts[to * n_limbs + l] = decay_const[from * n_limbs + l] % a.q[l];
+      }
+    if (int r = ensure_workspace(c, blob.size() / 4)) return r;
+    if (int r = launch_upload(c, c.ws, blob.data(), blob.size() / 4)) return r;
+    char *const ws = reinterpret_cast<char *>(c.ws);
+    a.left = reinterpret_cast<const CtctPair *>(ws);
+    a.right = a.left + (size_t)a.m * k;
+    a.out = reinterpret_cast<const CtctOut *>(ws + out_at);
+    a.consts = decay_const ? reinterpret_cast<const uint32_t *>(ws + consts_at) : nullptr;
     { int r_ = launch_ctct_gemm(c, a); c.mark("elementwise"); return r_; }
   });
 }

@@ -4,6 +4,30 @@
 // result, a plaintext polynomial or one constant per limb: the scores and the
 // weighted values of (decayed linear) attention over encrypted tokens. Words as
 // from cfhe_tensor_accum followed by a plaintext or constant product.
+//
+// For every word position this is an m x k by k x n matrix product over Z_q, a
+// small one with other operands at each position. Result by result each operand
+// word would be read once per result that it enters; here a block owns a tile of
+// results on C positions and every word is read once per tile. (The product of the
+// transposes is taken where m > n: the tensor product commutes, so m <= n below.)
+// Sixteen warps share the operand rows (C words of a polynomial) in a ring of
+// shared-memory stages. The stages of a block's tiles form one pipeline: copies
+// run ahead of the products over tile ends, and the pointers ahead of the copies.
+//
+// C is 64 or more: every row is another page, and an SM gets to a page that it did
+// not visit shortly before about every eight clocks, so rows of 64, 128 and 256
+// bytes come at 2.4, 4.5 and 6.2 TB/s at most (8.9 from L2).
+//
+// m <= 2: bound by reading R, whose words enter one or two results. m >= 3: bound by
+// the 32 x 32 + 64-bit multiply-adds, three instructions each here (20 a clock and
+// SM), so three products a term instead of four:
+//   b a' + a b' = (b + a)(b' + a') - b b' - a a'.
+// Tried instead for m >= 3, with the same result: bytes on the tensor cores
+// (tcgen05.mma wants 64 rows, a position has 2 n; mma.sync with operands split into
+// byte planes and seven 32-bit sums a result, which only fit tensor memory and leave
+// a tile of 4 x 8): 6.1 ms instead of 6.6 for 8 x 64 x 16 on 14 limbs, 6.6 instead of
+// 5.7 for 8 x 16 x 64 on 11. Double precision multiply-adds (56 a clock) need two a
+// product and conversions, as many instructions in all.
 #include "context.h"
 #include "kernels.h"
 #include "modmath.cuh"
@@ -11,42 +35,316 @@
 namespace cfhe {
 namespace {
 
-constexpr int kCcThreads = 256;
+// n / d for n below 2^31
+struct Divisor {
+  uint32_t d, mul, shift;
+  void set(uint32_t by) {
+    d = by;
+    shift = 31;
+    while ((1ull << (shift - 31)) < by) shift++;
+    mul = (uint32_t)(((1ull << shift) + by - 1) / by);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return (int)((uint64_t)(uint32_t)n * mul >> shift); }
+};
 
-// One result per block row: every operand word comes from memory (or L2) once
-// per result that it enters.
-__global__ void __launch_bounds__(kCcThreads) ctct_kernel(const __grid_constant__ CtctArgs a) {
+struct CtctPlan {
+  Divisor m_tiles, tiles;  // tiles along m, in all
+  int items;               // tiles x groups of positions x limbs
+};
+
+__device__ __forceinline__ uint32_t cc_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// Tile and first position of an item
+struct Where {
+  int i0, j0, l, position;
+};
+template <typename T>
+__device__ __forceinline__ Where where(const CtctPlan &p, int item) {
+  constexpr int kChunks = kN / T::C;
+  const int rest = p.tiles.quotient(item), tile = item - rest * (int)p.tiles.d;
+  const int tj = p.m_tiles.quotient(tile), ti = tile - tj * (int)p.m_tiles.d;
+  return {ti * T::kBm, tj * T::kBn, rest / kChunks, rest % kChunks * T::C};
+}
+
+// The asynchronous copies of a block. T: kBm x kBn results of a tile, C positions,
+// kTerms terms and kStages stages of the ring (kStage words each), kRowsT rows of a
+// term, those of R before kRowsR; entry(r, part): column or row of the tile and part
+// of row r; kWarps warps.
+template <typename T>
+struct Feed {
+  static constexpr int kThreads = 32 * T::kWarps;
+  static constexpr int kRows = T::kTerms * T::kRowsT, kPieces = T::C / 4;  // 16-byte pieces of a row
+  static constexpr int kCopies = (kRows * kPieces + kThreads - 1) / kThreads;
+  static constexpr int kPointers = (kRows + kThreads - 1) / kThreads;
+  const CtctArgs &a;
+  const CtctPlan &p;
+  uint32_t *const ring;
+  const uint32_t **const pointers;  // of the rows of 2 kStages stages, a ring of its own
+  const int tid, n_stages;
+  // pointers
+  int p_item, p_s = 0, p_slot = 0;
+  const uint32_t *const *p_at[kPointers];  // null: no such row
+  // copies
+  int c_item, c_s = 0, c_slot = 0, c_pslot = 0;
+  size_t c_at = 0;
+
+  __device__ __forceinline__ Feed(const CtctArgs &args, const CtctPlan &plan, uint32_t *smem)
+      : a(args), p(plan), ring(smem), pointers(reinterpret_cast<const uint32_t **>(smem + T::kStages * T::kStage)),
+        tid(threadIdx.x), n_stages((args.k + T::kTerms - 1) / T::kTerms), p_item(blockIdx.x), c_item(blockIdx.x) {}
+
+  // The pointers of one stage out of the tables, kStages stages before it is copied;
+  // a row that does not exist, or is past the last term, gets a null.
+  __device__ __forceinline__ void point() {
+#pragma unroll
+    for (int x = 0; x < kPointers; x++) {
+      const int row = tid + x * kThreads, t = row / T::kRowsT, r = row % T::kRowsT;
+      if (kRows % kThreads && row >= kRows) break;
+      const bool right = r < T::kRowsR;
+      const int width = right ? a.n : a.m;
+      if (p_s == 0) {
+        const Where w = where<T>(p, p_item);
+        int part;
+        const int e = T::entry(r, part) + (right ? w.j0 : w.i0);
+        const CtctPair *const tab = (right ? a.right : a.left) + (size_t)t * width + e;
+        p_at[x] = p_item < p.items && e < width ? reinterpret_cast<const uint32_t *const *>(tab) + part : nullptr;
+      }
+      const bool there = p_at[x] && p_s * T::kTerms + t < a.k;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(cc_smem(pointers + p_slot * kRows + row)),
+                   "l"(there ? (const void *)p_at[x] : (const void *)a.right), "r"(there ? 8 : 0)
+                   : "memory");
+      if (p_at[x]) p_at[x] += 2 * T::kTerms * width;
+    }
+    if (++p_s == n_stages) {
+      p_s = 0;
+      p_item += gridDim.x;
+    }
+    p_slot = p_slot + 1 == 2 * T::kStages ? 0 : p_slot + 1;
+  }
+  // One stage on its way. Nothing is copied where there is no row or term: what the
+  // ring holds there is not used.
+  __device__ __forceinline__ void copy() {
+    if (c_s == 0) {
+      const Where w = where<T>(p, c_item);
+      c_at = (size_t)w.l * kN + w.position + tid % kPieces * 4;
+    }
+    if (c_item < p.items) {
+      const uint32_t stage = cc_smem(ring + c_slot * T::kStage + tid % kPieces * 4);
+      const uint32_t *const *const from = pointers + c_pslot * kRows + tid / kPieces;
+#pragma unroll
+      for (int x = 0; x < kCopies; x++) {
+        const int row = tid / kPieces + x * (kThreads / kPieces);
+        if (kRows * kPieces % kThreads && row >= kRows) break;
+        const uint32_t *const src = from[x * (kThreads / kPieces)];
+        if (src)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage + 4 * row * T::C), "l"(src + c_at)
+                       : "memory");
+      }
+    }
+    if (++c_s == n_stages) {
+      c_s = 0;
+      c_item += gridDim.x;
+    }
+    c_slot = c_slot + 1 == T::kStages ? 0 : c_slot + 1;
+    c_pslot = c_pslot + 1 == 2 * T::kStages ? 0 : c_pslot + 1;
+  }
+  __device__ __forceinline__ void step() {
+    copy();
+    point();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void start() {  // pointers of kStages stages, copies of one less
+    for (int s = 0; s < T::kStages; s++) point();
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    for (int s = 0; s + 1 < T::kStages; s++) step();
+  }
+  __device__ __forceinline__ void arrived() {  // the oldest step, for every thread
+    asm volatile("cp.async.wait_group %0;" ::"n"(T::kStages - 2) : "memory");
+    __syncthreads();
+  }
+};
+
+// The words of result o: weighted, stored
+__device__ __forceinline__ void store_result(const CtctArgs &a, size_t o, int l, size_t at, uint32_t d0, uint32_t d1,
+                                             uint32_t d2, uint32_t q, uint32_t nq) {
+  const CtctOut to = a.out[o];
+  if (to.weight || a.consts) {
+    const uint32_t v = to.weight ? to.weight[at] : a.consts[o * a.n_limbs + l];
+    d0 = mont_mul(d0, v, q, nq);
+    d1 = mont_mul(d1, v, q, nq);
+    d2 = mont_mul(d2, v, q, nq);
+  }
+  to.d0[at] = d0;
+  to.d1[at] = d1;
+  to.d2[at] = d2;
+}
+
+// A product of residues is below q^2, a folded sum below q 2^32. For q <= 1.27e9
+// eight products may be added to a folded sum: the high word stays below
+// q + 8 q^2 / 2^32, which is below 2^32 and below 4 q, so subtracting 2 q and q
+// where they fit (two instructions each) folds it again. For larger q every second
+// product is followed by a fold.
+constexpr uint32_t kMaxQ8 = 1270000000u;
+
+template <bool EIGHT>
+__device__ __forceinline__ void fold_sum(uint64_t &s, uint32_t q) {
+  uint32_t hi = (uint32_t)(s >> 32);
+  if constexpr (EIGHT) hi = min(hi, hi - 2 * q);
+  hi = min(hi, hi - q);
+  s = ((uint64_t)hi << 32) | (uint32_t)s;
+}
+
+// Thread tiles of MT x NT results; WM warps along m, POSITIONS / 32 groups of
+// positions, the other warps along n; stages of TERMS terms
+template <int MT, int NT, int WM, int POSITIONS, int TERMS>
+struct SumsTile {
+  static constexpr int kWarps = 16, C = POSITIONS, kGroups = C / 32, kWn = kWarps / (kGroups * WM);
+  static constexpr int kBm = MT * WM, kBn = NT * kWn, kTerms = TERMS;
+  static constexpr int kRowsR = 2 * kBn, kRowsT = kRowsR + 2 * kBm, kStage = kTerms * kRowsT * C;
+  static constexpr int kFit = 220 * 1024 / (kStage * 4 + 2 * kTerms * kRowsT * 8);
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kBytes = kStages * (kStage * 4 + 2 * kTerms * kRowsT * 8);
+  static __device__ __forceinline__ int entry(int r, int &part) {
+    part = r & 1;
+    return (r < kRowsR ? r : r - kRowsR) >> 1;
+  }
+};
+__device__ __forceinline__ void mad_wide(uint64_t &s, uint32_t a, uint32_t b) {
+  asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(s) : "r"(a), "r"(b));
+}
+
+template <int MT, int NT, int WM, int POSITIONS, int TERMS, bool EIGHT>
+__global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant__ CtctArgs a,
+                                                                 const __grid_constant__ CtctPlan p) {
+  using T = SumsTile<MT, NT, WM, POSITIONS, TERMS>;
+  constexpr bool kThree = MT > 2;  // three products a term
+  extern __shared__ __align__(16) uint32_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   pdl_wait();
-  const int l = blockIdx.z, o = blockIdx.y, i = o / a.n, j = o % a.n;
-  const size_t at = (size_t)l * kN + blockIdx.x * kCcThreads + threadIdx.x;
-  const uint32_t q = a.q[l], nq = a.nqinv[l];
-  const uint64_t q32 = (uint64_t)q << 32;
-  const int mk = a.m * a.k, kn = a.k * a.n, mn = a.m * a.n;
-  const uint32_t *const *lb = a.table + i * a.k, *const *la = lb + mk;
-  const uint32_t *const *rb = a.table + 2 * mk + j, *const *ra = rb + kn;
-  const uint32_t *const *out = a.table + 2 * (mk + kn) + o;
-  uint64_t s0 = 0, s1 = 0, s2 = 0;
-  for (int t = 0; t < a.k; t++) {
-    const uint32_t xb = lb[t][at], xa = la[t][at], yb = rb[t * a.n][at], ya = ra[t * a.n][at];
-    mac_fold(s0, xb, yb, q32);
-    mac_fold(s1, xb, ya, q32);
-    mac_fold(s1, xa, yb, q32);
-    mac_fold(s2, xa, ya, q32);
+  Feed<T> feed(a, p, smem);
+  feed.start();
+  const int group = warp % T::kGroups, wj = warp / T::kGroups % T::kWn, wi = warp / (T::kGroups * T::kWn);
+  const int my_r = 2 * wj * NT * T::C + 32 * group + lane, my_l = (T::kRowsR + 2 * wi * MT) * T::C + 32 * group + lane;
+  int slot = 0;
+  for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+    const Where w = where<T>(p, item);
+    const int i0 = w.i0 + wi * MT, j0 = w.j0 + wj * NT;
+    const uint32_t q = a.q[w.l], nq = a.nqinv[w.l];
+    uint64_t s0[MT][NT], s1[MT][NT], s2[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) s0[i][j] = s1[i][j] = s2[i][j] = 0;
+    for (int s = 0; s < feed.n_stages; s++) {
+      feed.arrived();  // and all have left the stage before
+      feed.step();
+      const uint32_t *const stage = smem + slot * T::kStage;
+      slot = slot + 1 == T::kStages ? 0 : slot + 1;
+      if (i0 >= a.m || j0 >= a.n) continue;
+#pragma unroll
+      for (int u = 0; u < T::kTerms; u++) {
+        if (u > 0 && s * T::kTerms + u >= a.k) break;
+        const uint32_t *const lp = stage + my_l + u * T::kRowsT * T::C, *const rp = stage + my_r + u * T::kRowsT * T::C;
+        uint32_t lb[MT], la[MT], ls[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          lb[i] = lp[2 * i * T::C];
+          la[i] = lp[(2 * i + 1) * T::C];
+          if constexpr (kThree) ls[i] = add_mod(lb[i], la[i], q);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const uint32_t rb = rp[2 * j * T::C], ra = rp[(2 * j + 1) * T::C];
+          const uint32_t rs = kThree ? add_mod(rb, ra, q) : 0;
+#pragma unroll
+          for (int i = 0; i < MT; i++) {
+            mad_wide(s0[i][j], lb[i], rb);
+            if constexpr (kThree) {
+              mad_wide(s1[i][j], ls[i], rs);
+            } else {
+              mad_wide(s1[i][j], lb[i], ra);
+              mad_wide(s1[i][j], la[i], rb);
+              if constexpr (!EIGHT) fold_sum<false>(s1[i][j], q);
+            }
+            mad_wide(s2[i][j], la[i], ra);
+          }
+        }
+        // folds: after two products, or after eight
+        const int done = s * T::kTerms + u;
+        const bool fold = EIGHT ? done % 8 == 7 : done % 2 == 1, fold1 = kThree ? fold : EIGHT && done % 4 == 3;
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+            if (fold1) fold_sum<EIGHT>(s1[i][j], q);
+            if (fold) {
+              fold_sum<EIGHT>(s0[i][j], q);
+              fold_sum<EIGHT>(s2[i][j], q);
+            }
+          }
+      }
+    }
+    const size_t at = (size_t)w.l * kN + w.position + 32 * group + lane;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        if (i0 + i >= a.m || j0 + j >= a.n) continue;
+        fold_sum<EIGHT>(s0[i][j], q);
+        fold_sum<EIGHT>(s1[i][j], q);
+        fold_sum<EIGHT>(s2[i][j], q);
+        const uint32_t d0 = mont_reduce(s0[i][j], q, nq), d2 = mont_reduce(s2[i][j], q, nq);
+        uint32_t d1 = mont_reduce(s1[i][j], q, nq);
+        if constexpr (kThree) d1 = sub_mod(sub_mod(d1, d0, q), d2, q);
+        store_result(a, (size_t)(i0 + i) * a.n + j0 + j, w.l, at, d0, d1, d2, q, nq);
+      }
   }
-  uint32_t d[3] = {mont_reduce(s0, q, nq), mont_reduce(s1, q, nq), mont_reduce(s2, q, nq)};
-  if (a.weights || a.consts) {
-    const uint32_t w = a.weights ? out[3 * mn][at] : a.consts[(size_t)o * a.n_limbs + l];
-    for (int p = 0; p < 3; p++) d[p] = mont_mul(d[p], w, q, nq);
-  }
-  for (int p = 0; p < 3; p++) const_cast<uint32_t *>(out[p * mn])[at] = d[p];
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// ---- launches
+template <typename T, typename Kernel>
+int launch_tiles(const Context &ctx, const CtctArgs &a, Kernel kernel, PerDeviceOnce &once) {
+  if (int r = once.run(ctx.device, [&] {
+        CFHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kBytes));
+        return 0;
+      }))
+    return r;
+  CtctPlan p;
+  p.m_tiles.set((a.m + T::kBm - 1) / T::kBm);
+  p.tiles.set(p.m_tiles.d * ((a.n + T::kBn - 1) / T::kBn));
+  p.items = p.tiles.d * (kN / T::C) * a.n_limbs;
+  CFHE_CUDA(launch_kernel(ctx.use_pdl, kernel, dim3(min(p.items, ctx.num_sms)), dim3(32 * T::kWarps), T::kBytes,
+                          ctx.stream, a, p));
+  return 0;
+}
+
+template <int MT, int NT, int WM, int POSITIONS, int TERMS, bool EIGHT>
+int launch_sums(const Context &ctx, const CtctArgs &a) {
+  using T = SumsTile<MT, NT, WM, POSITIONS, TERMS>;
+  static_assert(T::kStages >= 3, "copies ahead of the products");
+  static PerDeviceOnce once;
+  return launch_tiles<T>(ctx, a, ctct_sums_kernel<MT, NT, WM, POSITIONS, TERMS, EIGHT>, once);
+}
+
+// Tiles of m x 32 (m <= 2), 4 x 16 or 8 x 8 results on 64 positions; few columns
+// leave warps for more positions.
+template <bool EIGHT>
+int launch(const Context &ctx, const CtctArgs &a) {
+  if (a.m == 1) return a.n > 8 ? launch_sums<1, 4, 1, 64, 2, EIGHT>(ctx, a) : launch_sums<1, 4, 1, 256, 2, EIGHT>(ctx, a);
+  if (a.m == 2) return a.n > 8 ? launch_sums<2, 4, 1, 64, 2, EIGHT>(ctx, a) : launch_sums<2, 4, 1, 256, 2, EIGHT>(ctx, a);
+  if (a.m <= 4) return a.n > 8 ? launch_sums<4, 2, 1, 64, 4, EIGHT>(ctx, a) : launch_sums<4, 2, 1, 128, 4, EIGHT>(ctx, a);
+  return launch_sums<4, 2, 2, 64, 8, EIGHT>(ctx, a);
 }
 
 }  // namespace
 
+// args.m <= args.n
 int launch_ctct_gemm(const Context &ctx, const CtctArgs &args) {
-  const dim3 grid(kN / kCcThreads, args.m * args.n, args.n_limbs), block(kCcThreads);
-  CFHE_CUDA(launch_kernel(ctx.use_pdl, ctct_kernel, grid, block, 0, ctx.stream, args));
+  uint32_t top = 0;
+  for (int l = 0; l < args.n_limbs; l++) top = max(top, args.q[l]);
+  if (int r = top <= kMaxQ8 ? launch<true>(ctx, args) : launch<false>(ctx, args)) return r;
   CFHE_CUDA(cudaGetLastError());
   return 0;
 }

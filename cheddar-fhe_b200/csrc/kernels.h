@@ -197,13 +197,20 @@ struct RotaryCall {
 int launch_rotary(const Context &ctx, const RotaryCall &call);
 
 // ctct_gemm.cu: D[i][j] = w[i][j] (*) sum_t L[i][t] (x) R[t][j], three parts
+struct CtctPair {
+  const uint32_t *b, *a;
+};
+struct CtctOut {
+  uint32_t *d0, *d1, *d2;
+  const uint32_t *weight;  // plaintext, or null
+};
 struct CtctArgs {
-  int m, k, n, n_limbs;
-  // device table: left b [m*k], left a, right b [k*n], right a, d0 [m*n], d1, d2,
-  // then weight plaintexts [m*n] where weights is 1
-  const uint32_t *const *table;
-  const uint32_t *consts;  // device, [m*n][n_limbs], or null
-  int weights;             // plaintext weights present
+  int m, k, n, n_limbs;    // m <= n
+  // device tables: the operands of term t at left[t * m + i], right[t * n + j],
+  // result (i, j) at out[i * n + j]
+  const CtctPair *left, *right;
+  const CtctOut *out;
+  const uint32_t *consts;  // constant weights [m * n][n_limbs] on the device, or null
   uint32_t q[kMaxLimbs], nqinv[kMaxLimbs];
 };
 int launch_ctct_gemm(const Context &ctx, const CtctArgs &args);

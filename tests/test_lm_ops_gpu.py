@@ -229,6 +229,61 @@ def test_ctct_gemm_largest_residues(engine40):
                 assert e.torch.all(d[:, :, p, l, 1::2] == f * odd % q), (k, l, p)
 
 
+def primes_below(bound, count):
+    """Primes of the ring (1 mod 2^17) below `bound`, largest first."""
+    out, q = [], (bound - 2) // (1 << 17) * (1 << 17) + 1
+    while len(out) < count:
+        if all(pow(a, q - 1, q) == 1 for a in (2, 3, 5, 7)) and all(q % d for d in range(3, 1 << 16, 2)):
+            out.append(q)
+        q -= 1 << 17
+    return out
+
+
+@pytest.mark.parametrize("bound", [1270000000, 1 << 31])
+def test_operators_at_the_largest_primes(pkg, bound):
+    """The largest prime with eight products between two folds of a sum, and the
+    largest there are (two): largest words, then random ones, in every kernel."""
+    main = primes_below(bound, 4)
+    aux = primes_below(1 << 29, 2)
+    e = pkg.Engine({"log_degree": 16, "main_primes": main, "terminal_primes": [], "auxiliary_primes": aux,
+                    "level_config": [[1, 0], [2, 0], [3, 0], [4, 0]], "additional_base": [0, 0]})
+    g = [0, 1]
+    q0 = int(e.primes[0])
+    assert bound - q0 < 1 << 24
+    for m, n in ((1, 3), (1, 20), (2, 7), (2, 33), (3, 5), (4, 17), (8, 9), (9, 6)):
+        for k in (1, 2, 7, 8, 9, 16, 17, 33):
+            left, right = e.empty(m, k, 2, 2, e.n), e.empty(k, n, 2, 2, e.n)
+            for l in range(2):
+                left[..., l, :] = int(e.primes[l]) - 1
+                right[..., l, :] = int(e.primes[l]) - 1
+            d = e.empty(m, n, 3, 2, e.n)
+            e.ctct_gemm_(d, left, right, g)
+            for l in range(2):
+                q = int(e.primes[l])
+                for p, f in enumerate((1, 2, 1)):
+                    assert e.torch.all(d[:, :, p, l] == f * k * pow(1 << 32, -1, q) % q), (m, n, k, l, p)
+        left, right = draw(e, m, g, m, 19, 2), draw(e, n, g, 19, n, 2)
+        w = constants(e, 3, g, m, n)
+        d = e.empty(m, n, 3, 2, e.n)
+        e.ctct_gemm_(d, left, right, g, decay=w)
+        assert e.torch.equal(d, want_ctct(e, left, right, g, w)), (m, n)
+    x = draw(e, 1, g, 2, 6, 2)
+    cos, sin = draw(e, 2, g, 3), draw(e, 3, g, 3)
+    y = e.torch.empty_like(x)
+    e.rotary_(y, x, cos, sin, g)
+    assert e.torch.equal(y, want_rotary(e, x, cos, sin, g, False))
+    w = np.ascontiguousarray(np.moveaxis(constants(e, 4, g, 6, 5), -1, 0))
+    w[:, 1:] = (np.array([int(e.primes[l]) - 1 for l in g], dtype=np.uint32))[:, None, None]
+    b, s = np.ascontiguousarray(constants(e, 5, g, 5).T), constants(e, 6, g)
+    r = draw(e, 7, g, 5, 2)
+    y = e.empty(5, 2, 2, e.n)
+    e.ctpt_project_(y, x[0], e.gemm_pack_weights(w, g), g, bias=b, residual=r, res_scale=s)
+    for j in range(5):
+        for l in range(2):
+            assert e.torch.equal(y[j, :, l], want_project(e, x[0], w, g, l, j, b, r, s)), (j, l)
+    e.close()
+
+
 def test_ctct_gemm_equals_tensor_accum(engine40):
     e = engine40
     g = list(e.level_limbs(3))
