@@ -867,24 +867,27 @@ int cfhe_ctpt_project(cfhe_context *h, uint32_t *const *yb, uint32_t *const *ya,
     const size_t bias_at = blob.w.size() * sizeof(uint32_t);
     if (bias)
       for (int l = 0; l < n_limbs; l++)
-        for (int j = 0; j < n_out; j++) blob.w.push_back(bias[(size_t)l * n_out + j] % c.q[gidx[l]]);
-    uint32_t scale[kMaxLimbs];
-    for (int l = 0; l < n_limbs; l++) {
-      const uint32_t q = c.q[gidx[l]];
-      scale[l] = res_scale ? res_scale[l] % q : (uint32_t)((1ull << 32) % q);
-    }
-    const size_t limb = (gemm_scratch_bytes(n_in) + 255) / 256 * 256;
-    const size_t scratch = gemm_packs_ahead(n_out, n_limbs) ? 2 * limb : limb;
+        for (int j = 0; j < n_out; j++)
+          blob.w.push_back((uint32_t)(((uint64_t)bias[(size_t)l * n_out + j] << 32) % c.q[gidx[l]]));
+    const size_t scratch = gemm_scratch_bytes(n_in) * project_buffers(n_in, n_out, n_limbs);
     if (int r = ensure_workspace(c, scratch / 4 + blob.w.size())) return r;
-    char *base = reinterpret_cast<char *>(c.ws), *tab = base + scratch;
-    uint8_t *const packed_x[2] = {(uint8_t *)base, scratch > limb ? (uint8_t *)base + limb : nullptr};
+    char *const tab = reinterpret_cast<char *>(c.ws) + scratch;
     if (int r = launch_upload(c, tab, blob.w.data(), blob.w.size())) return r;
-    for (int p = 0; p < 2; p++)
-      if (int r = launch_ctpt_project(c, (uint32_t *const *)(tab + y_at[p]), (const uint32_t *const *)(tab + x_at[p]),
-                                      (const uint8_t *)packed, packed_x, n_in, n_out,
-                                      bias && p == 0 ? (const uint32_t *)(tab + bias_at) : nullptr,
-                                      rb ? (const uint32_t *const *)(tab + r_at[p]) : nullptr, scale, gidx, n_limbs))
-        return r;
+    ProjectCall call;
+    for (int p = 0; p < 2; p++) {
+      call.x[p] = reinterpret_cast<const uint32_t *const *>(tab + x_at[p]);
+      call.y[p] = reinterpret_cast<uint32_t *const *>(tab + y_at[p]);
+      call.res[p] = rb ? reinterpret_cast<const uint32_t *const *>(tab + r_at[p]) : nullptr;
+    }
+    call.packed = static_cast<const uint8_t *>(packed);
+    call.scratch = reinterpret_cast<uint8_t *>(c.ws);
+    call.bias = bias ? reinterpret_cast<const uint32_t *>(tab + bias_at) : nullptr;
+    call.res_scale = res_scale;
+    call.n_in = n_in;
+    call.n_out = n_out;
+    call.n_limbs = n_limbs;
+    call.gidx = gidx;
+    if (int r = launch_ctpt_project(c, call)) return r;
     c.mark("gemm");
     return 0;
   });

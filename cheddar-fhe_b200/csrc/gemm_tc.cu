@@ -37,6 +37,7 @@
 //
 // Every barrier wait is bounded; a wait that runs out raises the context's
 // error flag and the CTA winds down without touching the accumulators.
+#include <algorithm>
 #include <vector>
 
 #include "context.h"
@@ -55,7 +56,7 @@ constexpr int kGmStages = 4;
 constexpr int kGmAStage = kGmTile * kGmStepBytes;   // 8 KiB
 constexpr int kGmBStage = kGmCols * kGmStepBytes;   // 16 KiB
 constexpr int kGmThreads = 192;     // warps 0-3 epilogue, warp 4 copies, warp 5 MMA
-constexpr int kGmSmem = kGmStages * (kGmAStage + kGmBStage) + 128;
+constexpr int kGmSmem = kGmStages * (kGmAStage + kGmBStage) + 128;  // and the barriers
 constexpr uint32_t kWaitHintNs = 2000;
 constexpr uint32_t kSpinLimit = 1u << 20;
 
@@ -74,11 +75,23 @@ struct GemmArgs {
   const uint32_t *const *x;
   size_t next_off;
   int n_in;
-  // projection (EPI): what joins an output word before it is stored; null where
-  // there is none. A residual's table holds a null for an output without one.
-  const uint32_t *const *res;  // n_out residual polynomials, multiplied by res_scale (M-form)
-  const uint32_t *bias;        // n_out words of this limb
-  uint32_t res_scale;
+};
+
+// A projection takes its limbs of both polynomials in groups, one launch for a group.
+// An entry is one limb of one polynomial, with what joins an output word before it
+// is stored.
+constexpr int kMaxGroup = 16;
+struct ProjectEntry {
+  const uint8_t *xp, *wp;
+  uint32_t *const *y;
+  const uint32_t *const *x;
+  const uint32_t *const *res;  // n_out residual polynomials, or null; a null among them: none
+  const uint32_t *bias;        // n_out words times 2^32 mod q, or null
+  size_t limb_off;
+  uint32_t q, nqinv, res_scale;  // res_scale in M-form
+};
+struct ProjectGroup {
+  ProjectEntry e[kMaxGroup];
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -151,7 +164,47 @@ __device__ __forceinline__ void store_chunk(uint8_t *xp, int k_chunks, int m_til
   *reinterpret_cast<uint4 *>(xp + ((size_t)m_tile * k_chunks + t) * (kGmTile * 16) + row * 16) = w;
 }
 
-template <bool EPI>
+// K step ks of a tile: D (128 x 256, s32) += A (128 x 64 u8) * B (64 x 256 u8), as two K = 32 instructions
+__device__ __forceinline__ void issue_step(uint32_t tmem, const uint8_t *sA, const uint8_t *sB, int s, bool first) {
+  const uint32_t idesc = (2u << 4) | ((uint32_t)(kGmCols >> 3) << 17) | ((uint32_t)(kGmTile >> 4) << 24);
+  constexpr uint32_t a_lbo = (kGmTile / 8) * 128, b_lbo = (kGmCols / 8) * 128;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const uint64_t da = smem_desc(smem_u32(sA + s * kGmAStage) + h * 2 * a_lbo, a_lbo, 128);
+    const uint64_t db = smem_desc(smem_u32(sB + s * kGmBStage) + h * 2 * b_lbo, b_lbo, 128);
+    const uint32_t acc = (!first || h > 0) ? 1u : 0u;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+// arrives at `bar` when the MMAs issued so far have been carried out
+__device__ __forceinline__ void commit_mma(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// V = d0 + d1 2^8 + d2 2^16 + d3 2^24, every d below 2^31
+__device__ __forceinline__ uint64_t join_planes(const uint32_t *d) {
+  return (uint64_t)d[0] + ((uint64_t)d[1] << 8) + ((uint64_t)d[2] << 16) + ((uint64_t)d[3] << 24);
+}
+
+// Units [u0, u1) of the next limb's packing, a unit being one K chunk of one tile
+// (128 threads, 2 KiB); `part` of `parts` groups of 128 threads takes its share
+__device__ __forceinline__ void pack_ahead(const GemmArgs &a, int u0, int u1, int row, int part, int parts) {
+  const int k_chunks = 4 * a.k_steps;
+  for (int u = u0 + 4 * part; u < u1; u += 4 * parts) {  // 16 loads a thread in flight
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (u + i < u1) w[i] = load_chunk(a.x, a.next_off, a.n_in, (u + i) / k_chunks, row, (u + i) % k_chunks);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (u + i < u1) store_chunk(a.xp_next, k_chunks, (u + i) / k_chunks, row, (u + i) % k_chunks, w[i]);
+  }
+}
+
 __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_constant__ GemmArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *sA = smem;                               // [stage][4][16][8][16]
@@ -160,6 +213,7 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
   uint64_t *full = bars, *empty = bars + kGmStages, *accum = bars + 2 * kGmStages;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kGmStages + 1);
   __shared__ int s_failed;
+  __shared__ uint32_t *s_y[kGmOutTile];  // this CTA's outputs
   const int tid = threadIdx.x, warp = tid >> 5;
   const int n_tile = blockIdx.x, m_tile = blockIdx.y;
   pdl_launch_dependents();
@@ -200,56 +254,32 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
       bulk_load(smem_u32(sB + s * kGmBStage), bp + (size_t)ks * kGmBStage, kGmBStage, smem_u32(full + s));
     }
   } else if (tid == 5 * 32) {
-    // ---- MMAs: D (128 x 256, s32) += A (128 x 64 u8) * B (64 x 256 u8) per stage, as two K = 32 instructions
-    const uint32_t idesc = (2u << 4) | ((uint32_t)(kGmCols >> 3) << 17) | ((uint32_t)(kGmTile >> 4) << 24);
-    constexpr uint32_t a_lbo = (kGmTile / 8) * 128, b_lbo = (kGmCols / 8) * 128;
-    bool ok = true;
-    for (int ks = 0; ks < a.k_steps && ok; ks++) {
+    // ---- MMAs
+    for (int ks = 0; ks < a.k_steps; ks++) {
       const int s = ks % kGmStages, round = ks / kGmStages;
       if (!mbar_wait(smem_u32(full + s), round & 1)) {
         atomicExch(a.error_flag, 1);
         atomicExch(&s_failed, 1);
-        ok = false;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const uint64_t da = smem_desc(smem_u32(sA + s * kGmAStage) + h * 2 * a_lbo, a_lbo, 128);
-        const uint64_t db = smem_desc(smem_u32(sB + s * kGmBStage) + h * 2 * b_lbo, b_lbo, 128);
-        const uint32_t acc = (ks > 0 || h > 0) ? 1u : 0u;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-            "l"(da), "l"(db), "r"(idesc), "r"(acc)
-            : "memory");
-      }
-      // the stage is free again once these MMAs have read it
-      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                       smem_u32(empty + s))
-                   : "memory");
+      issue_step(tmem, sA, sB, s, ks == 0);
+      commit_mma(smem_u32(empty + s));  // the stage is free again once these MMAs have read it
     }
     // accumulators complete (also on failure, so that the epilogue warps wake up)
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     smem_u32(accum))
-                 : "memory");
+    commit_mma(smem_u32(accum));
   } else if (warp < 4) {
-    // ---- meanwhile: this CTA's share of the next limb's packing, a unit being
-    // one K chunk of one tile (128 threads, 2 KiB)
+    // looked up output by output between the stores, the table costs a load's latency each time
+    if (tid < kGmOutTile) {
+      const int j = n_tile * kGmOutTile + tid;
+      s_y[tid] = j < a.n_out ? a.y[j] : nullptr;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    // ---- meanwhile: this CTA's share of the next limb's packing
     if (a.xp_next) {
-      const int k_chunks = 4 * a.k_steps, units = (int)gridDim.y * k_chunks;
+      const long long units = (long long)gridDim.y * 4 * a.k_steps;
       const int cta = blockIdx.y * gridDim.x + blockIdx.x, n_cta = gridDim.x * gridDim.y;
-      const int u0 = (int)((long long)units * cta / n_cta), u1 = (int)((long long)units * (cta + 1) / n_cta);
-      for (int u = u0; u < u1; u += 4) {  // 16 loads a thread in flight
-        uint4 w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (u + i < u1) w[i] = load_chunk(a.x, a.next_off, a.n_in, (u + i) / k_chunks, tid, (u + i) % k_chunks);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (u + i < u1) store_chunk(a.xp_next, k_chunks, (u + i) / k_chunks, tid, (u + i) % k_chunks, w[i]);
-      }
+      pack_ahead(a, (int)(units * cta / n_cta), (int)(units * (cta + 1) / n_cta), tid, 0, 1);
     }
     // ---- epilogue: thread = coefficient, 8 outputs (32 columns) per tensor-memory load
     const bool arrived = mbar_wait(smem_u32(accum), 0);
@@ -266,21 +296,8 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const int j = n_tile * kGmOutTile + j0 + e;
-          if (j < a.n_out) {
-            // V = d0 + d1 2^8 + d2 2^16 + d3 2^24, every d below 2^31
-            uint64_t v = (uint64_t)d[4 * e] + ((uint64_t)d[4 * e + 1] << 8) +
-                         ((uint64_t)d[4 * e + 2] << 16) + ((uint64_t)d[4 * e + 3] << 24);
-            if constexpr (EPI) {
-              // v < 2^23 q and the product below q 2^31: still one reduction
-              const uint32_t *r = a.res ? a.res[j] : nullptr;
-              if (r) v += (uint64_t)r[col] * a.res_scale;
-              const uint32_t y = mont_reduce(v, q, nq);
-              a.y[j][col] = a.bias ? add_mod(y, a.bias[j], q) : y;
-            } else {
-              a.y[j][col] = mont_reduce(v, q, nq);
-            }
-          }
+          uint32_t *const to = s_y[j0 + e];
+          if (to) to[col] = mont_reduce(join_planes(d + 4 * e), q, nq);
         }
       }
     }
@@ -288,6 +305,174 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 4)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kGmCols) : "memory");
+}
+
+// A projection: the same tiles, with residual and bias in the epilogue, by CTAs that
+// stay. A CTA walks a list of tiles (outputs fastest, then coefficients, then
+// entries); copies and, once the epilogue has fetched its accumulators, MMAs of the
+// next tile go on under the epilogue of the last. Eight epilogue warps: with a
+// residual a word takes some 35 instructions, so few inputs (32: two K steps a tile)
+// leave the epilogue the longer part. Against a CTA a tile: 32 x 64 on 3 limbs
+// 95 -> 82 us, 130 x 77 with a residual on 9 limbs 770 -> 690 us; 768 x 768 on 11
+// limbs takes 12.2 to 13.1 ms either way, at the power limit.
+constexpr int kPjWarps = 8, kPjThreads = 32 * (kPjWarps + 2), kPjOuts = kGmOutTile / 2;
+
+__global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_constant__ GemmArgs a,
+                                                                   const __grid_constant__ ProjectGroup group,
+                                                                   int n_tiles, int n_entries) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t *sA = smem, *sB = smem + kGmStages * kGmAStage;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kGmStages * (kGmAStage + kGmBStage));
+  uint64_t *full = bars, *empty = bars + kGmStages, *accum = bars + 2 * kGmStages, *drained = accum + 1;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_failed;
+  // the outputs of a tile, of two tiles in turn
+  __shared__ uint32_t *s_y[2][kGmOutTile];
+  __shared__ const uint32_t *s_res[2][kGmOutTile];
+  __shared__ uint32_t s_bias[2][kGmOutTile];
+  constexpr int kTilesM = kN / kGmTile;
+  const int tid = threadIdx.x, warp = tid >> 5, per_entry = n_tiles * kTilesM, tiles = per_entry * n_entries;
+  pdl_launch_dependents();
+  if (tid == 0) {
+    for (int s = 0; s < kGmStages; s++) {
+      mbar_init(smem_u32(full + s), 1);
+      mbar_init(smem_u32(empty + s), 1);
+    }
+    mbar_init(smem_u32(accum), 1);
+    mbar_init(smem_u32(drained), kPjWarps);
+    s_failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kPjWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(kGmCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  auto fail = [&] {
+    atomicExch(a.error_flag, 1);
+    atomicExch(&s_failed, 1);
+  };
+
+  if (tid == kPjWarps * 32) {
+    // ---- copies, running on from tile to tile
+    int s = 0, round = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      const int z = tile / per_entry, rest = tile % per_entry;
+      const uint8_t *ap = group.e[z].xp + (size_t)(rest / n_tiles) * a.k_steps * kGmAStage;
+      const uint8_t *bp = group.e[z].wp + (size_t)(rest % n_tiles) * a.k_steps * kGmBStage;
+      for (int ks = 0; ks < a.k_steps; ks++) {
+        if (round > 0 && !mbar_wait(smem_u32(empty + s), (round - 1) & 1)) {
+          fail();
+          ok = false;
+          break;
+        }
+        mbar_expect_tx(smem_u32(full + s), kGmAStage + kGmBStage);
+        bulk_load(smem_u32(sA + s * kGmAStage), ap + (size_t)ks * kGmAStage, kGmAStage, smem_u32(full + s));
+        bulk_load(smem_u32(sB + s * kGmBStage), bp + (size_t)ks * kGmBStage, kGmBStage, smem_u32(full + s));
+        if (++s == kGmStages) {
+          s = 0;
+          round++;
+        }
+      }
+    }
+  } else if (tid == (kPjWarps + 1) * 32) {
+    // ---- MMAs
+    int s = 0, round = 0, n = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, n++) {
+      if (n > 0) {
+        ok = mbar_wait(smem_u32(drained), (n - 1) & 1);
+        if (!ok) fail();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      for (int ks = 0; ks < a.k_steps && ok; ks++) {
+        ok = mbar_wait(smem_u32(full + s), round & 1);
+        if (!ok) {
+          fail();
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        issue_step(tmem, sA, sB, s, ks == 0);
+        commit_mma(smem_u32(empty + s));
+        if (++s == kGmStages) {
+          s = 0;
+          round++;
+        }
+      }
+      commit_mma(smem_u32(accum));  // also on failure, so that the epilogue warps wake up
+    }
+  } else if (warp < kPjWarps) {
+    // ---- epilogue: thread = coefficient and half of the tile's outputs
+    const int row = tid & 127, half = tid >> 7, lane = tid & 31;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 4 * half * kPjOuts;
+    int n = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, n++) {
+      const int z = tile / per_entry, rest = tile % per_entry, n_tile = rest % n_tiles;
+      const ProjectEntry &e = group.e[z];
+      const int b = n & 1;
+      if (tid < kGmOutTile) {
+        const int j = n_tile * kGmOutTile + tid;
+        s_y[b][tid] = j < a.n_out ? e.y[j] : nullptr;
+        s_res[b][tid] = e.res && j < a.n_out ? e.res[j] : nullptr;
+        s_bias[b][tid] = e.bias && j < a.n_out ? e.bias[j] : 0;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kPjWarps) : "memory");
+      // meanwhile: this tile's share of the next entry's packing (one entry a launch then)
+      if (a.xp_next) {
+        const long long units = (long long)kTilesM * 4 * a.k_steps;
+        pack_ahead(a, (int)(units * rest / per_entry), (int)(units * (rest + 1) / per_entry), row, half, 2);
+      }
+      // the residual words of this thread, on their way during the products
+      const size_t col = e.limb_off + (size_t)(rest / n_tiles) * kGmTile + row;
+      const bool res = e.res != nullptr;
+      uint32_t r[kPjOuts];
+      if (res) {
+#pragma unroll
+        for (int j = 0; j < kPjOuts; j++) {
+          const uint32_t *const from = s_res[b][half * kPjOuts + j];
+          r[j] = from ? from[col] : 0;
+        }
+      }
+      const bool arrived = mbar_wait(smem_u32(accum), n & 1);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (!arrived) fail();
+      if (!arrived || *(volatile int *)&s_failed) break;
+      const uint32_t q = e.q, nq = e.nqinv, res_scale = e.res_scale;
+#pragma unroll
+      for (int j0 = 0; j0 < kPjOuts; j0 += 8) {
+        uint32_t d[32];
+        tmem_ld32(lane_base + 4 * j0, d);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (j0 + 8 == kPjOuts) {  // the accumulators are in registers
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(drained)) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int o = half * kPjOuts + j0 + i;
+          uint32_t *const to = s_y[b][o];
+          if (to) {
+            // the planes give less than 2^23 q, the residual less than q 2^31 and the bias
+            // (times 2^32 mod q) less than q: still one reduction
+            uint64_t v = join_planes(d + 4 * i) + s_bias[b][o];
+            if (res) v += (uint64_t)r[j0 + i] * res_scale;
+            to[col] = mont_reduce(v, q, nq);
+          }
+        }
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == kPjWarps)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kGmCols) : "memory");
 }
 
@@ -300,6 +485,17 @@ __global__ void __launch_bounds__(256) gemm_pack_kernel(uint8_t *xp, const uint3
   pdl_wait();
   const int c = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
   store_chunk(xp, k_chunks, c >> 7, c & 127, t, load_chunk(x, limb_off, n_in, c >> 7, c & 127, t));
+}
+
+// The same for the entries of a group
+__global__ void __launch_bounds__(256) project_pack_kernel(const __grid_constant__ ProjectGroup group, int n_in,
+                                                           int k_chunks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const ProjectEntry &e = group.e[blockIdx.z];
+  const int c = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+  store_chunk(const_cast<uint8_t *>(e.xp), k_chunks, c >> 7, c & 127, t,
+              load_chunk(e.x, e.limb_off, n_in, c >> 7, c & 127, t));
 }
 
 }  // namespace
@@ -339,7 +535,7 @@ void gemm_pack_weights_limb(uint8_t *out, const uint32_t *w, int n_in, int n_out
 // x, y: device tables of n_in / n_out polynomial pointers ([n_limbs][N] words
 // each); wp: packed weights, limb after limb; scratch: two buffers for one limb
 // of packed activations each (gemm_scratch_bytes), the second may be null.
-size_t gemm_scratch_bytes(int n_in) {
+size_t gemm_scratch_bytes(int n_in) {  // a multiple of 8 KiB
   const int k_steps = (4 * n_in + kGmStepBytes - 1) / kGmStepBytes;
   return (size_t)(kN / kGmTile) * k_steps * kGmAStage;
 }
@@ -354,13 +550,11 @@ bool gemm_packs_ahead(int n_out, int n_limbs) {
   return n_limbs > 1 && (n_out + kGmOutTile - 1) / kGmOutTile >= 3;
 }
 
-template <bool EPI>
-static int launch_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
-                       uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs,
-                       const uint32_t *const *res, const uint32_t *bias, const uint32_t *res_scale) {
+int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
+                     uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs) {
   static PerDeviceOnce once;
   if (int r = once.run(c.device, [] {
-        CFHE_CUDA(cudaFuncSetAttribute(gemm_tc_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem));
+        CFHE_CUDA(cudaFuncSetAttribute(gemm_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem));
         return 0;
       }))
     return r;
@@ -396,28 +590,75 @@ static int launch_gemm(const Context &c, uint32_t *const *y, const uint32_t *con
     a.q = c.q[gidx[l]];
     a.nqinv = c.nqinv[gidx[l]];
     a.error_flag = c.d_error_flag;
-    a.res = res;
-    a.bias = bias ? bias + (size_t)l * n_out : nullptr;
-    a.res_scale = res_scale ? res_scale[l] : 0;
-    CFHE_CUDA(launch_kernel(c.use_pdl, gemm_tc_kernel<EPI>, dim3(n_tiles, kN / kGmTile), dim3(kGmThreads), kGmSmem,
+    CFHE_CUDA(launch_kernel(c.use_pdl, gemm_tc_kernel, dim3(n_tiles, kN / kGmTile), dim3(kGmThreads), kGmSmem,
                             c.stream, a));
   }
   CFHE_CUDA(cudaGetLastError());
   return 0;
 }
 
-int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
-                     uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs) {
-  return launch_gemm<false>(c, y, x, wp, scratch, n_in, n_out, gidx, n_limbs, nullptr, nullptr, nullptr);
+// ---- projections: the limbs of both polynomials, limb after limb, so that the
+// polynomials of a limb find its weights in L2.
+//
+// From three output tiles on an entry's activations are packed inside the products
+// of the entry before (two buffers); with fewer, entries go in groups of up to 64 MiB
+// of packed activations, two launches a group (packing inside the products was slower:
+// 130 x 77 on 9 limbs 1.00 instead of 0.78 ms).
+int project_buffers(int n_in, int n_out, int n_limbs) {
+  if (gemm_packs_ahead(n_out, 2 * n_limbs)) return 2;
+  const size_t fit = ((size_t)64 << 20) / gemm_scratch_bytes(n_in);
+  return (int)std::min({(size_t)kMaxGroup, (size_t)2 * n_limbs, std::max(fit, (size_t)1)});
 }
 
-// One polynomial of a projection: res a device table of n_out pointers (null
-// entries: no residual) or null, bias [n_limbs][n_out] on the device or null,
-// res_scale [n_limbs] on the host.
-int launch_ctpt_project(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
-                        uint8_t *const *scratch, int n_in, int n_out, const uint32_t *bias,
-                        const uint32_t *const *res, const uint32_t *res_scale, const int *gidx, int n_limbs) {
-  return launch_gemm<true>(c, y, x, wp, scratch, n_in, n_out, gidx, n_limbs, res, bias, res_scale);
+int launch_ctpt_project(const Context &c, const ProjectCall &p) {
+  static PerDeviceOnce once;
+  if (int r = once.run(c.device, [] {
+        CFHE_CUDA(cudaFuncSetAttribute(project_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kGmSmem));
+        return 0;
+      }))
+    return r;
+  const int k_steps = (4 * p.n_in + kGmStepBytes - 1) / kGmStepBytes;
+  const int n_tiles = (p.n_out + kGmOutTile - 1) / kGmOutTile;
+  const int entries = 2 * p.n_limbs, buffers = project_buffers(p.n_in, p.n_out, p.n_limbs);
+  const bool ahead = gemm_packs_ahead(p.n_out, entries);
+  const size_t w_limb = gemm_packed_weight_bytes(p.n_in, p.n_out), x_bytes = gemm_scratch_bytes(p.n_in);
+  const int group = ahead ? 1 : buffers;
+  for (int e0 = 0; e0 < entries; e0 += group) {
+    const int n = std::min(group, entries - e0);
+    ProjectGroup g;
+    for (int i = 0; i < n; i++) {
+      const int e = e0 + i, l = e / 2, poly = e % 2;
+      const uint32_t prime = c.q[p.gidx[l]];
+      g.e[i] = {p.scratch + (size_t)(e % buffers) * x_bytes,
+                p.packed + (size_t)l * w_limb,
+                p.y[poly],
+                p.x[poly],
+                p.res[poly],
+                poly == 0 && p.bias ? p.bias + (size_t)l * p.n_out : nullptr,
+                (size_t)l * kN,
+                prime,
+                c.nqinv[p.gidx[l]],
+                p.res_scale ? p.res_scale[l] % prime : (uint32_t)((1ull << 32) % prime)};
+    }
+    if (!ahead || e0 == 0)
+      CFHE_CUDA(launch_kernel(c.use_pdl, project_pack_kernel, dim3(kN / 256, 4 * k_steps, n), dim3(256), 0, c.stream, g,
+                              p.n_in, 4 * k_steps));
+    GemmArgs a = {};
+    a.k_steps = k_steps;
+    a.n_out = p.n_out;
+    a.error_flag = c.d_error_flag;
+    if (ahead && e0 + 1 < entries) {
+      a.xp_next = p.scratch + (size_t)((e0 + 1) % buffers) * x_bytes;
+      a.x = p.x[(e0 + 1) % 2];
+      a.next_off = (size_t)((e0 + 1) / 2) * kN;
+      a.n_in = p.n_in;
+    }
+    CFHE_CUDA(launch_kernel(c.use_pdl, project_tc_kernel, dim3(std::min(n_tiles * (kN / kGmTile) * n, 2 * c.num_sms)),
+                            dim3(kPjThreads), kGmSmem, c.stream, a, g, n_tiles, n));
+  }
+  CFHE_CUDA(cudaGetLastError());
+  return 0;
 }
 
 }  // namespace cfhe

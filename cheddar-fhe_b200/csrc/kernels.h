@@ -174,9 +174,22 @@ bool gemm_packs_ahead(int n_out, int n_limbs);
 void gemm_pack_weights_limb(uint8_t *out, const uint32_t *w, int n_in, int n_out, uint32_t q);
 int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
                      uint8_t *const *scratch, int n_in, int n_out, const int *gidx, int n_limbs);
-int launch_ctpt_project(const Context &c, uint32_t *const *y, const uint32_t *const *x, const uint8_t *wp,
-                        uint8_t *const *scratch, int n_in, int n_out, const uint32_t *bias,
-                        const uint32_t *const *res, const uint32_t *res_scale, const int *gidx, int n_limbs);
+// A projection with its epilogue. x, y, res: device tables of n_in / n_out pointers
+// for the b and the a polynomial (res null: none, a null entry: none for that
+// output); bias [n_limbs][n_out] words times 2^32
+// mod q on the device or null; res_scale [n_limbs] on
+// the host or null (1); scratch: project_buffers x gemm_scratch_bytes.
+struct ProjectCall {
+  uint32_t *const *y[2];
+  const uint32_t *const *x[2], *const *res[2];
+  const uint8_t *packed;
+  uint8_t *scratch;
+  const uint32_t *bias, *res_scale;
+  int n_in, n_out, n_limbs;
+  const int *gidx;
+};
+int project_buffers(int n_in, int n_out, int n_limbs);
+int launch_ctpt_project(const Context &c, const ProjectCall &call);
 // upload.cu: `words` host words to the device through kernel parameters
 int launch_upload(const Context &c, void *dst, const void *src, size_t words);
 
