@@ -1201,6 +1201,64 @@ class Context : public std::enable_shared_from_this<Context<word>> {
                                  b2.data(), a2.data(), t0 > 0, g.data(), g.size()));
     }
   }
+  // res[i * n + j] = (decay[i * n + j] *) sum_t a[i * k + t] * b[t * n + j], m x n
+  // unrelinearised three-part products of an m x k and a k x n matrix of ciphertexts
+  // on one level (without aux primes), in one call that reads every operand word once
+  // per tile of results (cfhe_ctct_gemm): the scores and the weighted values of
+  // attention over encrypted tokens. decay: one plaintext or one constant per result
+  // (linear attention's decay and mask), or nothing. Words as from MultSumUnsafe per
+  // result, then Mult with its plaintext or constant. No counterpart in the reference.
+  void MultMatrixUnsafe(std::vector<Ct> &res, const std::vector<const Ct *> &a, const std::vector<const Ct *> &b,
+                        int m, int k, int n, const std::vector<const Pt *> &decay = {}) const {
+    MatrixProduct(res, a, b, m, k, n, decay, nullptr);
+  }
+  void MultMatrixUnsafe(std::vector<Ct> &res, const std::vector<const Ct *> &a, const std::vector<const Ct *> &b,
+                        int m, int k, int n, const std::vector<Const> &decay) const {
+    AssertTrue((int)decay.size() == m * n, "MultMatrixUnsafe: one constant per result is needed");
+    MatrixProduct(res, a, b, m, k, n, {}, &decay);
+  }
+  // Rotary positions: rows of 2 `pairs` features each (x[row * 2 pairs + feature]),
+  // pair i = features (2i, 2i + 1), or (i, i + pairs) with halves:
+  //   (u, v) -> (cos[i] u - sin[i] v, sin[i] u + cos[i] v),
+  // unrescaled (cfhe_rotary, cfhe_rotary_token). cos, sin: a plaintext per pair, or a
+  // constant per pair where every slot is at the same position. res holds none of x.
+  // No counterpart in the reference.
+  void Rotary(std::vector<Ct> &res, const std::vector<const Ct *> &x, int pairs, bool halves,
+              const std::vector<const Pt *> &cos, const std::vector<const Pt *> &sin) const {
+    AssertTrue((int)cos.size() == pairs && (int)sin.size() == pairs, "Rotary: one cosine and sine per pair");
+    std::vector<const word *> c, s;
+    for (int i = 0; i < pairs; i++) {
+      AssertSameNP(*x.at(0), *cos[i]);
+      AssertSameNP(*x[0], *sin[i]);
+      AssertSameScale(cos[i]->GetScale(), cos[0]->GetScale());
+      AssertSameScale(sin[i]->GetScale(), cos[0]->GetScale());
+      c.push_back(cos[i]->mx_.data());
+      s.push_back(sin[i]->mx_.data());
+    }
+    std::vector<word *> y;
+    std::vector<const word *> in;
+    const auto g = RotaryOperands(res, x, pairs, cos.at(0)->GetScale(), y, in);
+    CheckAbi(cfhe_rotary(h_, y.data(), in.data(), (int)(in.size() / (2 * pairs)), pairs, halves, c.data(), s.data(),
+                         g.data(), g.size()));
+  }
+  void Rotary(std::vector<Ct> &res, const std::vector<const Ct *> &x, int pairs, bool halves,
+              const std::vector<Const> &cos, const std::vector<Const> &sin) const {
+    AssertTrue((int)cos.size() == pairs && (int)sin.size() == pairs, "Rotary: one cosine and sine per pair");
+    std::vector<word> c, s;
+    for (int i = 0; i < pairs; i++) {
+      AssertSameNP(*x.at(0), cos[i]);
+      AssertSameNP(*x[0], sin[i]);
+      AssertSameScale(cos[i].GetScale(), cos[0].GetScale());
+      AssertSameScale(sin[i].GetScale(), cos[0].GetScale());
+      c.insert(c.end(), cos[i].cx_.begin(), cos[i].cx_.end());
+      s.insert(s.end(), sin[i].cx_.begin(), sin[i].cx_.end());
+    }
+    std::vector<word *> y;
+    std::vector<const word *> in;
+    const auto g = RotaryOperands(res, x, pairs, cos.at(0).GetScale(), y, in);
+    CheckAbi(cfhe_rotary_token(h_, y.data(), in.data(), (int)(in.size() / (2 * pairs)), pairs, halves, c.data(),
+                               s.data(), g.data(), g.size()));
+  }
   void MultUnsafe(Ct &res, const Ct &a, const Pt &b, int level = -1) const {
     const NPInfo a_np = a.GetNP(), b_np = b.GetNP();
     if (level == -1) level = Min(param_.NPToLevel(a_np), param_.NPToLevel(b_np));
@@ -1515,6 +1573,79 @@ class Context : public std::enable_shared_from_this<Context<word>> {
   }
 
  protected:
+  void MatrixProduct(std::vector<Ct> &res, const std::vector<const Ct *> &a, const std::vector<const Ct *> &b, int m,
+                     int k, int n, const std::vector<const Pt *> &pt, const std::vector<Const> *consts) const {
+    AssertTrue(m > 0 && k > 0 && n > 0 && (int)a.size() == m * k && (int)b.size() == k * n,
+               "MultMatrixUnsafe: bad operand lists");
+    AssertTrue(pt.empty() || (int)pt.size() == m * n, "MultMatrixUnsafe: one plaintext per result is needed");
+    const NPInfo np = a[0]->GetNP();
+    AssertTrue(np.num_aux_ == 0, "MultMatrixUnsafe should be only used for ciphertexts without aux primes");
+    int slots = 0;
+    std::vector<const word *> p[4];
+    for (int side = 0; side < 2; side++)
+      for (const Ct *x : side ? b : a) {
+        AssertFalse(x->HasRx(), "Relinearization required before MultMatrixUnsafe");
+        AssertTrue(x->GetNP() == np, "MultMatrixUnsafe: operands on different levels");
+        AssertSameScale(x->GetScale(), (side ? b : a)[0]->GetScale());
+        slots = Max(slots, x->GetNumSlots());
+        p[2 * side].push_back(x->bx_.data());
+        p[2 * side + 1].push_back(x->ax_.data());
+      }
+    double scale = a[0]->GetScale() * b[0]->GetScale();
+    std::vector<const word *> w;
+    std::vector<word> c;
+    for (const Pt *x : pt) {
+      AssertTrue(x->GetNP() == np, "MultMatrixUnsafe: a plaintext on another level");
+      AssertSameScale(x->GetScale(), pt[0]->GetScale());
+      w.push_back(x->mx_.data());
+    }
+    if (consts)
+      for (const Const &x : *consts) {
+        AssertTrue(x.GetNP() == np, "MultMatrixUnsafe: a constant on another level");
+        AssertSameScale(x.GetScale(), consts->at(0).GetScale());
+        c.insert(c.end(), x.cx_.begin(), x.cx_.end());
+      }
+    if (!pt.empty()) scale *= pt[0]->GetScale();
+    if (consts) scale *= consts->at(0).GetScale();
+    std::vector<Ct> out;
+    std::vector<word *> d[3];
+    for (int o = 0; o < m * n; o++) {
+      out.emplace_back(np, true);
+      out[o].SetScale(scale);
+      out[o].SetNumSlots(slots);
+      d[0].push_back(out[o].bx_.data());
+      d[1].push_back(out[o].ax_.data());
+      d[2].push_back(out[o].rx_.data());
+    }
+    const auto g = param_.GetLimbIndices(np);
+    CheckAbi(cfhe_ctct_gemm(h_, d[0].data(), d[1].data(), d[2].data(), p[0].data(), p[1].data(), p[2].data(),
+                            p[3].data(), m, k, n, pt.empty() ? nullptr : w.data(), consts ? c.data() : nullptr, g.data(),
+                            g.size()));
+    res = std::move(out);
+  }
+  // results of Rotary, pointers of results and inputs: the rows' b polynomials, then their a
+  std::vector<int> RotaryOperands(std::vector<Ct> &res, const std::vector<const Ct *> &x, int pairs, double scale,
+                                  std::vector<word *> &y, std::vector<const word *> &in) const {
+    AssertTrue(pairs > 0 && !x.empty() && x.size() % (2 * (size_t)pairs) == 0, "Rotary: rows of 2 pairs features");
+    const NPInfo np = x[0]->GetNP();
+    AssertTrue(np.num_aux_ == 0, "Rotary should be only used for ciphertexts without aux primes");
+    std::vector<Ct> out;
+    for (const Ct *c : x) {
+      AssertFalse(c->HasRx(), "Relinearization required before Rotary");
+      AssertTrue(c->GetNP() == np, "Rotary: operands on different levels");
+      AssertSameScale(c->GetScale(), x[0]->GetScale());
+      out.emplace_back(np);
+      out.back().SetScale(c->GetScale() * scale);
+      out.back().SetNumSlots(c->GetNumSlots());
+    }
+    for (int poly = 0; poly < 2; poly++)
+      for (size_t i = 0; i < x.size(); i++) {
+        in.push_back(poly ? x[i]->ax_.data() : x[i]->bx_.data());
+        y.push_back(poly ? out[i].ax_.data() : out[i].bx_.data());
+      }
+    res = std::move(out);
+    return param_.GetLimbIndices(np);
+  }
   template <typename A, typename B>
   void AssertSameNP(const A &a, const B &b) const {
     AssertTrue(a.GetNP() == b.GetNP(), "NP mismatch");

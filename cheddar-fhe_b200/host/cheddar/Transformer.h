@@ -73,6 +73,22 @@ struct TransformerConfig {
   double gelu_range = 4.0;             // bound on the feed-forward pre-activation
   double ln_eps = 1e-5;
   int exp_degree = 15, inv_degree = 63, rsqrt_degree = 63, gelu_degree = 31;
+  // Linear attention with a decay for each head instead of softmax attention: token t
+  // takes decay^(t - u) (q_t . k_u) / sqrt(head_dim) of token u's value for every
+  // u <= t, nothing of the tokens behind it, without a normaliser (no exponential, no
+  // reciprocal, no bootstrap of a denominator). One decay in (0, 1] per head; empty:
+  // softmax attention, every token over all tokens.
+  std::vector<double> decay;
+  // Rotary positions on queries and keys: rotary_pairs[a] pairs of a head's features
+  // follow axis a, one axis after the other (text: one axis; video: time, height,
+  // width), features past them keep their values; rotary_positions[a][t] is token t's
+  // position on it. Pair i of an axis of n turns by position * rotary_base^(-i / n).
+  // Empty: none. Pairs are features (2i, 2i + 1), or (i, i + head_dim / 2) with
+  // rotary_halves.
+  std::vector<int> rotary_pairs;
+  std::vector<std::vector<double>> rotary_positions;
+  double rotary_base = 10000.0;
+  bool rotary_halves = false;
   bool pair_boot = true;  // bootstrap two real ciphertexts as one complex one
   int workers = 4;        // host threads (and streams) of the per-ciphertext stages
   static TransformerConfig BertBase() { return TransformerConfig{}; }
@@ -154,6 +170,27 @@ struct TransformerPolys {
   }
 };
 
+// Angle of every pair of a head's features at every token, [pair][token]: pairs
+// follow the axes in turn, those past the last axis stay (angle 0).
+inline std::vector<std::vector<double>> RotaryAngles(const std::vector<int> &pairs_of_axis,
+                                                     const std::vector<std::vector<double>> &positions, double base,
+                                                     int pairs, int tokens) {
+  AssertTrue(pairs_of_axis.size() == positions.size(), "Rotary: one list of positions per axis is needed");
+  std::vector<std::vector<double>> angles;
+  for (size_t axis = 0; axis < positions.size(); axis++) {
+    AssertTrue((int)positions[axis].size() == tokens && pairs_of_axis[axis] >= 0,
+               "Rotary: one position per token and axis is needed");
+    for (int i = 0; i < pairs_of_axis[axis]; i++) {
+      const double rate = std::pow(base, -(double)i / pairs_of_axis[axis]);
+      angles.emplace_back();
+      for (double p : positions[axis]) angles.back().push_back(p * rate);
+    }
+  }
+  AssertTrue((int)angles.size() <= pairs, "Rotary: the axes have more pairs than a head");
+  angles.resize(pairs, std::vector<double>(tokens, 0.0));
+  return angles;
+}
+
 // A plaintext matrix encoded on the limbs of one level and packed for the
 // tensor-core contraction.
 template <typename word>
@@ -212,6 +249,50 @@ class PlainMatrix {
     CheckAbi(cfhe_ctpt_gemm(ctx.h_, yb.data(), xb.data(), packed_.data(), n_in_, n_out_, g_.data(), (int)g_.size()));
     CheckAbi(cfhe_ctpt_gemm(ctx.h_, ya.data(), xa.data(), packed_.data(), n_in_, n_out_, g_.data(), (int)g_.size()));
   }
+  // y[j] = sum_k w[k][j] x[k] + bias[j] (+ one * residual[j]) in one call
+  // (cfhe_ctpt_project), not rescaled: bias in real numbers, `one` a constant that
+  // brings the residuals (at the level of x) to the scale of the product
+  void Project(const Context<word> &ctx, std::vector<Ct> &y, const std::vector<const Ct *> &x,
+               const std::vector<double> &bias, const std::vector<const Ct *> &residual = {},
+               const Constant<word> *one = nullptr) const {
+    AssertTrue((int)x.size() == n_in_ && (int)bias.size() == n_out_, "PlainMatrix: wrong input or bias count");
+    AssertTrue(residual.empty() ? one == nullptr : (int)residual.size() == n_out_ && one != nullptr,
+               "PlainMatrix: residuals go with their constant, one per output");
+    const NPInfo np = ctx.param_.LevelToNP(level_);
+    const double scale = x[0]->GetScale() * scale_;
+    std::vector<const word *> xp[2], rp[2];
+    for (const Ct *c : x) {
+      AssertTrue(c->GetNP() == np && !c->HasRx(), "PlainMatrix: input at the wrong level");
+      xp[0].push_back(c->bx_.data());
+      xp[1].push_back(c->ax_.data());
+    }
+    for (const Ct *c : residual) {
+      AssertTrue(c->GetNP() == np && !c->HasRx() && one->GetNP() == np, "PlainMatrix: residual at the wrong level");
+      ctx.AssertSameScale(c->GetScale() * one->GetScale(), scale);
+      rp[0].push_back(c->bx_.data());
+      rp[1].push_back(c->ax_.data());
+    }
+    std::vector<word> b((size_t)g_.size() * n_out_);
+    for (int j = 0; j < n_out_; j++) {
+      Constant<word> k;
+      ctx.encoder().EncodeConstant(k, level_, scale, bias[j]);
+      for (size_t l = 0; l < g_.size(); l++) b[l * n_out_ + j] = k.cx_[l];
+    }
+    y.clear();
+    y.reserve(n_out_);
+    std::vector<word *> yp[2];
+    for (int j = 0; j < n_out_; j++) {
+      y.emplace_back(np);
+      y[j].SetScale(scale);
+      y[j].SetNumSlots(x[0]->GetNumSlots());
+      yp[0].push_back(y[j].bx_.data());
+      yp[1].push_back(y[j].ax_.data());
+    }
+    CheckAbi(cfhe_ctpt_project(ctx.h_, yp[0].data(), yp[1].data(), xp[0].data(), xp[1].data(), packed_.data(), n_in_,
+                               n_out_, b.data(), residual.empty() ? nullptr : rp[0].data(),
+                               residual.empty() ? nullptr : rp[1].data(), one ? one->cx_.data() : nullptr, g_.data(),
+                               (int)g_.size()));
+  }
   // 8-bit multiply-accumulates of one Apply (both polynomials, all limbs)
   double Int8Macs(int degree) const { return 2.0 * g_.size() * 16.0 * n_in_ * (double)n_out_ * degree; }
 
@@ -220,6 +301,78 @@ class PlainMatrix {
   double scale_;
   std::vector<int> g_;
   DeviceVector<word> packed_;
+};
+
+// Linear attention with a decay, token by token: keys and values of the tokens so far
+// are kept, one ciphertext per feature and token, every slot another sequence. A new
+// token's query meets all of them in one product of ciphertexts, weighted by
+// decay^age:  o = sum_u decay^(t - u) (q . k_u) v_u. (The D x D state of the recurrent
+// form would lose a level with every token, since its update multiplies ciphertexts;
+// the sum over the kept tokens stays at three levels.)
+//
+// Positions are turned with Context::Rotary before Append and Attend, where wanted.
+template <typename word>
+class DecayedTokens {
+  using Ct = Ciphertext<word>;
+
+ public:
+  DecayedTokens(ConstContextPtr<word> ctx, int head_dim, double decay)
+      : ctx_{std::move(ctx)}, dim_{head_dim}, decay_{decay} {
+    AssertTrue(head_dim > 0 && decay > 0.0 && decay <= 1.0, "DecayedTokens: a decay in (0, 1] is needed");
+  }
+  int Tokens() const { return (int)keys_.size() / dim_; }
+  // k, v: head_dim ciphertexts of the newest token, on one level; the values are
+  // brought down to the level that the scores will have, two below
+  void Append(std::vector<Ct> k, const std::vector<const Ct *> &v) {
+    AssertTrue((int)k.size() == dim_ && (int)v.size() == dim_, "DecayedTokens: one ciphertext per feature");
+    const int level = ctx_->param_.NPToLevel(k[0].GetNP());
+    AssertTrue(keys_.empty() || k[0].GetNP() == keys_[0].GetNP(), "DecayedTokens: keys on different levels");
+    AssertTrue(level >= 3, "DecayedTokens: a token takes three levels");
+    for (auto &c : k) keys_.push_back(std::move(c));
+    for (const Ct *c : v) {
+      Ct low;
+      ctx_->LevelDown(low, *c, level - 2);
+      values_.push_back(std::move(low));
+    }
+  }
+  // o: head_dim ciphertexts, three levels below q and the keys; scale_by multiplies
+  // every score (1 / sqrt(head_dim), say). The newest kept token counts as age 0.
+  void Attend(std::vector<Ct> &o, const std::vector<const Ct *> &q, const EvaluationKey<word> &mult,
+              double scale_by = 1.0) const {
+    const int n = Tokens();
+    AssertTrue((int)q.size() == dim_, "DecayedTokens: one ciphertext per feature");
+    if (n == 0) Fail("DecayedTokens: no token is kept");
+    const int level = ctx_->param_.NPToLevel(q[0]->GetNP());
+    std::vector<const Ct *> k, v;
+    for (int d = 0; d < dim_; d++)
+      for (int u = 0; u < n; u++) k.push_back(&keys_[(size_t)u * dim_ + d]);
+    for (const Ct &c : values_) v.push_back(&c);
+    const auto &p = ctx_->param_;
+    const double scale = p.GetScale(level - 2) * p.GetRescalePrimeProd(level - 1) * p.GetRescalePrimeProd(level) /
+                         (q[0]->GetScale() * keys_[0].GetScale());
+    std::vector<Constant<word>> decay(n);
+    for (int u = 0; u < n; u++)
+      ctx_->encoder().EncodeConstant(decay[u], level, scale, scale_by * std::pow(decay_, n - 1 - u));
+    std::vector<Ct> raw, w(n);
+    ctx_->MultMatrixUnsafe(raw, q, k, 1, dim_, n, decay);
+    std::vector<const Ct *> left;
+    for (int u = 0; u < n; u++) {
+      Ct once;
+      ctx_->RelinearizeRescale(once, raw[u], mult);
+      ctx_->Rescale(w[u], once);
+      left.push_back(&w[u]);
+    }
+    ctx_->MultMatrixUnsafe(raw, left, v, 1, n, dim_);
+    o.clear();
+    o.resize(dim_);
+    for (int d = 0; d < dim_; d++) ctx_->RelinearizeRescale(o[d], raw[d], mult);
+  }
+
+ private:
+  ConstContextPtr<word> ctx_;
+  int dim_;
+  double decay_;
+  std::vector<Ct> keys_, values_;
 };
 
 template <typename word>
@@ -239,6 +392,12 @@ class EncryptedTransformerLayer {
     AssertTrue(cfg.seq_len % cfg.baby == 0, "Transformer: baby must divide seq_len");
     slots_ = ctx_->param_.degree_ / 2;
     AssertTrue(slots_ % cfg.seq_len == 0, "Transformer: seq_len must divide the slot count");
+    AssertTrue(cfg.decay.empty() || (int)cfg.decay.size() == cfg.heads, "Transformer: one decay per head is needed");
+    for (double d : cfg.decay) AssertTrue(d > 0.0 && d <= 1.0, "Transformer: decays lie in (0, 1]");
+    if (!cfg.rotary_pairs.empty() || !cfg.rotary_positions.empty()) {
+      AssertTrue(cfg.head_dim % 2 == 0, "Transformer: rotary positions need an even head_dim");
+      angles_ = RotaryAngles(cfg.rotary_pairs, cfg.rotary_positions, cfg.rotary_base, cfg.head_dim / 2, cfg.seq_len);
+    }
     lane_ = slots_ / cfg.seq_len;
     main_ = ctx_;
     cfhe_context *current = detail::CurrentHandle();
@@ -283,7 +442,8 @@ class EncryptedTransformerLayer {
     std::vector<Ct> qkv;
     {
       // Q is pre-divided by sqrt(head_dim) * score_range: the score ciphertexts hold s / score_range
-      const double qs = 1.0 / (std::sqrt((double)D) * cfg_.score_range);
+      // (linear attention: by sqrt(head_dim), they hold s)
+      const double qs = 1.0 / (std::sqrt((double)D) * (Linear() ? 1.0 : cfg_.score_range));
       // columns of this rank's heads only: Q, K and V of head h are features h D .. (h+1) D - 1
       std::vector<int> cols;
       for (int part = 0; part < 3; part++)
@@ -310,12 +470,21 @@ class EncryptedTransformerLayer {
     }
     Mark("QKV projection");
     if (probe_) probe_("qkv", qkv, 1.0);
+    if (!angles_.empty()) {
+      TurnPositions(qkv, head0, head1);
+      Mark("rotary positions");
+      if (probe_) probe_("rotary positions", qkv, 1.0);
+    }
     std::vector<Ct> o_un(H), stat(head1 - head0);
-    for (int h = head0; h < head1; h++) AttentionHead(h, qkv, o_un, stat[h - head0], evk);
-    qkv.clear();
-    Mark("scores, exponentials, weighted values");
     std::vector<Ct> o(H);
-    {
+    if (Linear()) {
+      for (int h = head0; h < head1; h++) LinearAttentionHead(h, qkv, o, evk);
+      qkv.clear();
+      Mark("linear attention");
+    } else {
+      for (int h = head0; h < head1; h++) AttentionHead(h, qkv, o_un, stat[h - head0], evk);
+      qkv.clear();
+      Mark("scores, exponentials, weighted values");
       BootAll(stat, evk, true);
       for (int h = head0; h < head1; h++) {
         Ct p;
@@ -327,8 +496,8 @@ class EncryptedTransformerLayer {
         });
       }
       o_un.clear();
+      Mark("softmax normaliser");
     }
-    Mark("softmax normaliser");
     if (world > 1) {
       AllGather(o, [&](int j) { return BlockOwner(heads, j / D); });
       Mark("all-gather: attention outputs");
@@ -342,9 +511,15 @@ class EncryptedTransformerLayer {
       for (int j = res0; j < res1; j++) cols.push_back(j);
       if (!m_wo_) m_wo_ = MakeMatrix(Columns(Centred(w_.wo, H, H, 1.0 / A), H, H, cols), H, cols.size(), o[0]);
       y1.resize(H);
-      Project(y1, *m_wo_, Pointers(o), Select(CentredBias(w_.bo, 1.0 / A), cols), cols);
-      o.clear();
-      AddCentredResidual(y1, x, res0, res1);
+      if (Linear()) {
+        ProjectWithResidual(y1, *m_wo_, Pointers(o), Select(CentredBias(w_.bo, 1.0 / A), cols), x, cols);
+        o.clear();
+        SubtractMean(y1, x, Level(y1[res0]) + 1, res0, res1);
+      } else {
+        Project(y1, *m_wo_, Pointers(o), Select(CentredBias(w_.bo, 1.0 / A), cols), cols);
+        o.clear();
+        AddCentredResidual(y1, x, res0, res1);
+      }
     }
     Mark("output projection, residual");
     if (probe_) probe_("centred sum 1", y1, A);
@@ -408,8 +583,10 @@ class EncryptedTransformerLayer {
       for (int f = 0; f < F; f++)
         for (int j = 0; j < H; j++) bias[j] += 0.5 * w_.b1[f] * w_.w2[(size_t)f * H + j];
       for (int j = 0; j < H; j++) bias[j] += w_.b2[j];
-      Project(y2, *m_w2_, Pointers(act), Select(CentredBias(bias, 1.0 / A), cols), cols);
-      act.clear();
+      if (!Linear()) {
+        Project(y2, *m_w2_, Pointers(act), Select(CentredBias(bias, 1.0 / A), cols), cols);
+        act.clear();
+      }
       // residual and linear part of the GELU in one projection of z: (I + W1 W2 / 2)^T z, centred
       if (!m_res_) {
         const auto t0 = std::chrono::steady_clock::now();
@@ -430,13 +607,18 @@ class EncryptedTransformerLayer {
       }
       std::vector<Ct> lin(H);
       Project(lin, *m_res_, Pointers(z), std::vector<double>(cols.size(), 0.0), cols);
-      const int ly = Level(y2[res0]);
-      ParallelFor(res1 - res0, [&](const ConstContextPtr<word> &cx, int i) {
-        const int j = res0 + i;
-        Ct low;  // lin[j] belongs to another item's pool: it is read here and freed after the loop
-        cx->LevelDown(low, lin[j], ly);
-        cx->Add(y2[j], y2[j], low);
-      });
+      if (Linear()) {
+        ProjectWithResidual(y2, *m_w2_, Pointers(act), Select(CentredBias(bias, 1.0 / A), cols), lin, cols);
+        act.clear();
+      } else {
+        const int ly = Level(y2[res0]);
+        ParallelFor(res1 - res0, [&](const ConstContextPtr<word> &cx, int i) {
+          const int j = res0 + i;
+          Ct low;  // lin[j] belongs to another item's pool: it is read here and freed after the loop
+          cx->LevelDown(low, lin[j], ly);
+          cx->Add(y2[j], y2[j], low);
+        });
+      }
     }
     z.clear();
     Mark("feed-forward projection 2, residual");
@@ -545,7 +727,10 @@ class EncryptedTransformerLayer {
     std::vector<Ct> raw;
     ctx_->Synchronize();
     const auto t0 = std::chrono::steady_clock::now();
-    m.Apply(*ctx_, raw, x);
+    if (Linear())
+      m.Project(*ctx_, raw, x, bias);
+    else
+      m.Apply(*ctx_, raw, x);
     ctx_->Synchronize();
     gemm_s_ += std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
     gemm_macs_ += m.Int8Macs(ctx_->param_.degree_);
@@ -556,9 +741,47 @@ class EncryptedTransformerLayer {
     ParallelFor((int)raw.size(), [&](const ConstContextPtr<word> &c, int j) {
       Ct &dst = y[out_index.empty() ? j : out_index[j]];
       c->Rescale(dst, raw[j]);
-      AddConst(c, dst, bias[j]);
+      if (!Linear()) AddConst(c, dst, bias[j]);
     });
   }
+  // y[cols[c]] = rescale(W x + bias + residual[cols[c]]): bias and residual join the
+  // product before its rescale; the residual comes from its own level
+  void ProjectWithResidual(std::vector<Ct> &y, const PlainMatrix<word> &m, const std::vector<const Ct *> &x,
+                           const std::vector<double> &bias, const std::vector<Ct> &residual,
+                           const std::vector<int> &cols) {
+    const int l = m.level();
+    AssertTrue(Level(*x[0]) == l, "Transformer: the matrix was prepared for another level");
+    const double product = Canon(l - 1) * ctx_->param_.GetRescalePrimeProd(l);
+    ctx_->AssertSameScale(x[0]->GetScale() * m.scale(), product);
+    std::vector<Ct> low(cols.size()), raw;
+    std::vector<const Ct *> res(cols.size());
+    ParallelFor((int)cols.size(), [&](const ConstContextPtr<word> &c, int i) {
+      AssertTrue(Level(residual[cols[i]]) >= l, "Transformer: the residual must not sit below the block's output");
+      c->LevelDown(low[i], residual[cols[i]], l);
+    });
+    for (size_t i = 0; i < cols.size(); i++) res[i] = &low[i];
+    Const one;
+    ctx_->encoder().EncodeConstant(one, l, product / low[0].GetScale(), 1.0);
+    ctx_->Synchronize();
+    const auto t0 = std::chrono::steady_clock::now();
+    m.Project(*ctx_, raw, x, bias, res, &one);
+    ctx_->Synchronize();
+    gemm_s_ += std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
+    gemm_macs_ += m.Int8Macs(ctx_->param_.degree_);
+    ParallelFor((int)raw.size(),
+                [&](const ConstContextPtr<word> &c, int j) { c->Rescale(y[cols[j]], raw[j]); });
+  }
+  // y[j] -= mean_j x[j] for j in [lo, hi), the mean brought down to `level` and
+  // rescaled to the level of y
+  void SubtractMean(std::vector<Ct> &y, const std::vector<Ct> &x, int level, int lo, int hi) {
+    Ct sum, low, mean;
+    ctx_->Copy(sum, x[0]);
+    for (size_t j = 1; j < x.size(); j++) ctx_->Add(sum, sum, x[j]);
+    ctx_->LevelDown(low, sum, level);
+    MultConstRescale(main_, mean, low, 1.0 / x.size());
+    ParallelFor(hi - lo, [&](const ConstContextPtr<word> &c, int i) { c->Sub(y[lo + i], y[lo + i], mean); });
+  }
+  bool Linear() const { return !cfg_.decay.empty(); }
 
   // ---- ranks: contiguous blocks, the first n % world ranks hold one more
   std::pair<int, int> Block(int n, int rank) const { return BlockOfRank(n, group_->world(), rank); }
@@ -701,16 +924,19 @@ class EncryptedTransformerLayer {
         const int g = 1 + i / D, d = i % D;
         RotateTokens(c, qg[g][d], Q(d), -g * nb, evk);
       });
+      std::vector<Ct> acc;  // of the main context, freed after the loop
+      {
+        std::vector<const Ct *> left, right;
+        for (int g = 0; g < ng; g++)
+          for (int d = 0; d < D; d++) left.push_back(g ? &qg[g][d] : &Q(d));
+        for (int d = 0; d < D; d++)
+          for (int b = 0; b < nb; b++) right.push_back(&kb[d][b]);
+        ctx_->MultMatrixUnsafe(acc, left, right, ng, D, nb);
+      }
       ParallelFor(T, [&](const Cx &c, int r) {
-        const int g = r / nb, b = r % nb;
-        Ct acc, u;
-        std::vector<const Ct *> left(D), right(D);
-        for (int d = 0; d < D; d++) {
-          left[d] = g ? &qg[g][d] : &Q(d);
-          right[d] = &kb[d][b];
-        }
-        c->MultSumUnsafe(acc, left, right);
-        c->RelinearizeRescale(u, acc, mult);
+        const int g = r / nb;
+        Ct u;
+        c->RelinearizeRescale(u, acc[r], mult);
         if (g) {
           Ct rot;
           RotateTokens(c, rot, u, g * nb, evk);
@@ -728,7 +954,7 @@ class EncryptedTransformerLayer {
     }
     // o_d[t] = sum_g rot_{g nb}( sum_b rot_{-g nb}(e_{g nb + b}) * rot_b(V_d) )[t]
     const int le = Level(e[0]);
-    std::vector<std::vector<Ct>> vb(D), eg(ng), part(ng);
+    std::vector<std::vector<Ct>> vb(D), eg(ng);
     ParallelFor(D, [&](const Cx &c, int d) {
       Ct low;
       c->LevelDown(low, V(d), le);
@@ -739,27 +965,149 @@ class EncryptedTransformerLayer {
       const int g = 1 + i / nb, b = i % nb;
       RotateTokens(c, eg[g][b], e[g * nb + b], -g * nb, evk);
     });
+    std::vector<const Ct *> left;
+    for (int g = 0; g < ng; g++)
+      for (int b = 0; b < nb; b++) left.push_back(g ? &eg[g][b] : &e[b]);
+    WeightedValues(h, left, vb, o_un, evk);
+  }
+
+  // o[h D + d] = sum_g rot_{g nb}( sum_b weights[g nb + b] * vb[d][b] ), the weights
+  // turned back by their giant step, vb the baby rotations of the values
+  void WeightedValues(int h, const std::vector<const Ct *> &weights, const std::vector<std::vector<Ct>> &vb,
+                      std::vector<Ct> &o, const EvkMap<word> &evk) {
+    const int D = cfg_.head_dim, nb = cfg_.baby, ng = cfg_.seq_len / nb;
+    const Evk &mult = evk.GetMultiplicationKey();
+    using Cx = ConstContextPtr<word>;
+    std::vector<Ct> acc;  // of the main context, freed after the loop
+    {
+      std::vector<const Ct *> right;
+      for (int b = 0; b < nb; b++)
+        for (int d = 0; d < D; d++) right.push_back(&vb[d][b]);
+      ctx_->MultMatrixUnsafe(acc, weights, right, ng, nb, D);
+    }
+    std::vector<std::vector<Ct>> part(ng);
     for (int g = 0; g < ng; g++) part[g].resize(D);
     ParallelFor(ng * D, [&](const Cx &c, int i) {
       const int g = i / D, d = i % D;
-      Ct acc, t;
-      std::vector<const Ct *> left(nb), right(nb);
-      for (int b = 0; b < nb; b++) {
-        left[b] = g ? &eg[g][b] : &e[b];
-        right[b] = &vb[d][b];
-      }
-      c->MultSumUnsafe(acc, left, right);
-      c->RelinearizeRescale(t, acc, mult);
+      Ct t;
+      c->RelinearizeRescale(t, acc[i], mult);
       if (g)
         RotateTokens(c, part[g][d], t, g * nb, evk);
       else
         part[0][d] = std::move(t);
     });
     ParallelFor(D, [&](const Cx &c, int d) {
-      Ct &dst = o_un[h * D + d];
+      Ct &dst = o[h * D + d];
       c->Copy(dst, part[0][d]);
       for (int g = 1; g < ng; g++) c->Add(dst, dst, part[g][d]);
     });
+  }
+
+  // Queries and keys of heads [head0, head1) turned by their tokens' positions, one
+  // level down. Values stay where they are: they are brought down with the weights.
+  void TurnPositions(std::vector<Ct> &qkv, int head0, int head1) {
+    const int H = cfg_.hidden, D = cfg_.head_dim, T = cfg_.seq_len, P = D / 2;
+    const int l = Level(qkv[head0 * D]);
+    const double scale = Canon(l - 1) * ctx_->param_.GetRescalePrimeProd(l) / qkv[head0 * D].GetScale();
+    if (cos_.empty() || ctx_->param_.NPToLevel(cos_[0].GetNP()) != l) {
+      cos_.clear();
+      sin_.clear();
+      for (int i = 0; i < P; i++) {
+        std::vector<Complex> c(slots_), s(slots_);
+        for (int t = 0; t < T; t++)
+          for (int b = 0; b < lane_; b++) {
+            c[t * lane_ + b] = Complex(std::cos(angles_[i][t]), 0.0);
+            s[t * lane_ + b] = Complex(std::sin(angles_[i][t]), 0.0);
+          }
+        cos_.emplace_back();
+        sin_.emplace_back();
+        ctx_->encoder().Encode(cos_.back(), l, scale, c, 0);
+        ctx_->encoder().Encode(sin_.back(), l, scale, s, 0);
+      }
+    }
+    std::vector<const Plaintext<word> *> c, s;
+    for (int i = 0; i < P; i++) {
+      c.push_back(&cos_[i]);
+      s.push_back(&sin_[i]);
+    }
+    std::vector<int> where;
+    for (int part = 0; part < 2; part++)
+      for (int j = head0 * D; j < head1 * D; j++) where.push_back(part * H + j);
+    std::vector<const Ct *> x;
+    for (int j : where) x.push_back(&qkv[j]);
+    std::vector<Ct> raw;
+    ctx_->Rotary(raw, x, P, cfg_.rotary_halves, c, s);
+    ParallelFor((int)where.size(), [&](const ConstContextPtr<word> &cx, int i) {
+      Ct t;
+      cx->Rescale(t, raw[i]);
+      cx->Copy(qkv[where[i]], t);  // into the buffers of the main context
+    });
+  }
+
+  // Head h of linear attention: the weight of offset r = g nb + b, turned back by its
+  // giant step, is decay^(t - u) s_(t, u) at token t + g nb with u = t + r (mod T), and
+  // 0 unless u <= t. Decay and mask come with the scores' product, so that the weights
+  // take one more rescale and nothing else, and since nothing else is done to them in
+  // the order of the tokens, they are not turned forth and back.
+  void LinearAttentionHead(int h, const std::vector<Ct> &qkv, std::vector<Ct> &o, const EvkMap<word> &evk) {
+    const int H = cfg_.hidden, D = cfg_.head_dim, T = cfg_.seq_len, nb = cfg_.baby, ng = T / nb;
+    const Evk &mult = evk.GetMultiplicationKey();
+    using Cx = ConstContextPtr<word>;
+    std::vector<Ct> weights(T);
+    {
+      std::vector<std::vector<Ct>> kb(D), qg(ng);
+      ParallelFor(D, [&](const Cx &c, int d) { BabyRotations(c, kb[d], qkv[H + h * D + d], evk); });
+      for (int g = 1; g < ng; g++) qg[g].resize(D);
+      ParallelFor((ng - 1) * D, [&](const Cx &c, int i) {
+        const int g = 1 + i / D, d = i % D;
+        RotateTokens(c, qg[g][d], qkv[h * D + d], -g * nb, evk);
+      });
+      std::vector<const Ct *> left, right;
+      for (int g = 0; g < ng; g++)
+        for (int d = 0; d < D; d++) left.push_back(g ? &qg[g][d] : &qkv[h * D + d]);
+      for (int d = 0; d < D; d++)
+        for (int b = 0; b < nb; b++) right.push_back(&kb[d][b]);
+      const int l = Level(*left[0]);
+      const double scale = Canon(l - 2) * ctx_->param_.GetRescalePrimeProd(l - 1) *
+                           ctx_->param_.GetRescalePrimeProd(l) / (left[0]->GetScale() * right[0]->GetScale());
+      std::vector<const Plaintext<word> *> decay;
+      for (int r = 0; r < T; r++) decay.push_back(&DecayMask(cfg_.decay[h], r, l, scale));
+      std::vector<Ct> acc;  // of the main context, freed after the loop
+      ctx_->MultMatrixUnsafe(acc, left, right, ng, D, nb, decay);
+      ParallelFor(T, [&](const Cx &c, int r) {
+        Ct once;
+        c->RelinearizeRescale(once, acc[r], mult);
+        c->Rescale(weights[r], once);
+      });
+    }
+    const int lw = Level(weights[0]);
+    std::vector<std::vector<Ct>> vb(D);
+    ParallelFor(D, [&](const Cx &c, int d) {
+      Ct low;
+      c->LevelDown(low, qkv[2 * H + h * D + d], lw);
+      BabyRotations(c, vb[d], low, evk);
+    });
+    WeightedValues(h, Pointers(weights), vb, o, evk);
+  }
+
+  // decay^(t - u) at slot (t + g nb) B + b for the tokens t that see token u = t + r
+  // (mod T), 0 for the others
+  const Plaintext<word> &DecayMask(double decay, int r, int level, double scale) {
+    const auto key = std::make_tuple(decay, r, level, scale);
+    auto it = decays_.find(key);
+    if (it == decays_.end()) {
+      const int T = cfg_.seq_len, turned = r / cfg_.baby * cfg_.baby;
+      std::vector<Complex> msg(slots_);
+      for (int t = 0; t < T; t++) {
+        const int u = (t + r) % T;
+        const double w = u <= t ? std::pow(decay, t - u) : 0.0;
+        for (int b = 0; b < lane_; b++) msg[(size_t)((t + turned) % T) * lane_ + b] = Complex(w, 0.0);
+      }
+      Plaintext<word> pt;
+      ctx_->encoder().Encode(pt, level, scale, msg, 0);
+      it = decays_.emplace(key, std::move(pt)).first;
+    }
+    return it->second;
   }
 
   // z[j] = gamma_j y[j] / sqrt(var + eps) + beta_j / act_div for centred y
@@ -902,6 +1250,9 @@ class EncryptedTransformerLayer {
   std::unique_ptr<PlainMatrix<word>> m_qkv_, m_wo_, m_w1_, m_w2_, m_res_;
   Probe probe_;
   std::map<std::tuple<int, double, double>, Plaintext<word>> masks_;
+  std::map<std::tuple<double, int, int, double>, Plaintext<word>> decays_;  // decay, offset, level, scale
+  std::vector<std::vector<double>> angles_;                                 // of the rotary positions, [pair][token]
+  std::vector<Plaintext<word>> cos_, sin_;                                  // encoded at the level they are used on
   std::vector<double> mask_signs_;
   std::vector<std::pair<std::string, double>> stage_s_;
   std::chrono::steady_clock::time_point last_;
