@@ -870,8 +870,9 @@ int cfhe_ctpt_project(cfhe_context *h, uint32_t *const *yb, uint32_t *const *ya,
         for (int j = 0; j < n_out; j++)
           blob.w.push_back((uint32_t)(((uint64_t)bias[(size_t)l * n_out + j] << 32) % c.q[gidx[l]]));
     const size_t scratch = gemm_scratch_bytes(n_in) * project_buffers(n_in, n_out, n_limbs);
-    if (int r = ensure_workspace(c, scratch / 4 + blob.w.size())) return r;
-    char *const tab = reinterpret_cast<char *>(c.ws) + scratch;
+    uint32_t *memory = nullptr;
+    if (int r = call_memory(c, scratch / 4 + blob.w.size(), &memory)) return r;
+    char *const tab = reinterpret_cast<char *>(memory) + scratch;
     if (int r = launch_upload(c, tab, blob.w.data(), blob.w.size())) return r;
     ProjectCall call;
     for (int p = 0; p < 2; p++) {
@@ -880,7 +881,7 @@ int cfhe_ctpt_project(cfhe_context *h, uint32_t *const *yb, uint32_t *const *ya,
       call.res[p] = rb ? reinterpret_cast<const uint32_t *const *>(tab + r_at[p]) : nullptr;
     }
     call.packed = static_cast<const uint8_t *>(packed);
-    call.scratch = reinterpret_cast<uint8_t *>(c.ws);
+    call.scratch = reinterpret_cast<uint8_t *>(memory);
     call.bias = bias ? reinterpret_cast<const uint32_t *>(tab + bias_at) : nullptr;
     call.res_scale = res_scale;
     call.n_in = n_in;
@@ -975,9 +976,10 @@ int cfhe_ctct_gemm(cfhe_context *h, uint32_t *const *d0, uint32_t *const *d1, ui
         for (int l = 0; decay_const && l < n_limbs; l++)
           consts[to * n_limbs + l] = decay_const[from * n_limbs + l] % a.q[l];
       }
-    if (int r = ensure_workspace(c, blob.size() / 4)) return r;
-    if (int r = launch_upload(c, c.ws, blob.data(), blob.size() / 4)) return r;
-    char *const ws = reinterpret_cast<char *>(c.ws);
+    uint32_t *memory = nullptr;
+    if (int r = call_memory(c, blob.size() / 4, &memory)) return r;
+    if (int r = launch_upload(c, memory, blob.data(), blob.size() / 4)) return r;
+    char *const ws = reinterpret_cast<char *>(memory);
     a.left = reinterpret_cast<const CtctPair *>(ws);
     a.right = a.left + (size_t)a.m * k;
     a.out = reinterpret_cast<const CtctOut *>(ws + out_at);

@@ -115,6 +115,7 @@ struct Context {
   // workspace arena for pipeline temporaries (grown on demand)
   uint32_t *ws = nullptr;
   size_t ws_words = 0;
+  std::vector<void *> graph_blocks;  // memory of captured calls (call_memory), kept until the context goes
 
   // Device allocator behind cfhe_malloc / cfhe_free. Requests of 1 MiB and
   // more (polynomials) are carved, best fit, out of slabs of 1 GiB taken from
@@ -172,6 +173,10 @@ int build_plans(Context &ctx);
 int noalloc_prepare(int device);  // noalloc.cu: materialise the built-in scratch array on the current device
 void free_plans(Context &ctx);
 int ensure_workspace(Context &ctx, size_t words);
+// Device memory for the tables and temporaries of one call: the workspace, or, while
+// the stream is being captured, a block of its own, so that a graph neither shares
+// memory with another graph or a later call nor loses it when the workspace grows.
+int call_memory(Context &ctx, size_t words, uint32_t **out);
 
 void set_error(const std::string &msg);
 const std::string &get_error();

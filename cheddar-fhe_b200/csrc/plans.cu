@@ -197,6 +197,8 @@ void free_plans(Context &c) {
   if (c.ws) cudaFree(c.ws);
   c.ws = nullptr;
   c.ws_words = 0;
+  for (void *p : c.graph_blocks) cudaFree(p);
+  c.graph_blocks.clear();
   if (c.d_error_flag) cudaFree(c.d_error_flag);
   c.d_error_flag = nullptr;
   if (c.order_event) cudaEventDestroy(c.order_event);
@@ -223,6 +225,26 @@ int ensure_workspace(Context &c, size_t words) {
   c.ws_words = 0;
   CFHE_CUDA(cudaMalloc(&c.ws, words * sizeof(uint32_t)));
   c.ws_words = words;
+  return 0;
+}
+
+int call_memory(Context &c, size_t words, uint32_t **out) {
+  cudaStreamCaptureStatus status;
+  CFHE_CUDA(cudaStreamIsCapturing(c.stream, &status));
+  if (status == cudaStreamCaptureStatusNone) {
+    const int r = ensure_workspace(c, words);
+    *out = c.ws;
+    return r;
+  }
+  c.graph_blocks.reserve(c.graph_blocks.size() + 1);
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // an allocation is not part of the capture
+  CFHE_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  void *p = nullptr;
+  const cudaError_t err = cudaMalloc(&p, words * sizeof(uint32_t));
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  CFHE_CUDA(err);
+  c.graph_blocks.push_back(p);
+  *out = static_cast<uint32_t *>(p);
   return 0;
 }
 

@@ -403,6 +403,48 @@ def test_captured_and_replayed(pkg, params40):
     e.close()
 
 
+def test_graphs_share_no_memory(pkg, params40):
+    """Two graphs captured from one fresh context, the second one's calls larger; an
+    eager call that needs more than either (and regrows the workspace) between the
+    captures and the replays; replays of both at once on two streams."""
+    e = pkg.Engine(params40)
+    torch, g = e.torch, PRIMES[:2]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    jobs = []
+    for i, (m, k, n) in enumerate([(1, 5, 3), (3, 9, 40)]):
+        left, right = draw(e, 160 + i, g, m, k, 2), draw(e, 170 + i, g, k, n, 2)
+        x, w = draw(e, 180 + i, g, 3 + i, 2), constants(e, 190 + i, g, 3 + i, 4)
+        packed = e.gemm_pack_weights(np.ascontiguousarray(np.moveaxis(w, -1, 0)), g)
+        jobs.append((left, right, constants(e, 200 + i, g, m, n), e.empty(m, n, 3, 2, e.n), x, packed,
+                     np.moveaxis(w, -1, 0), e.empty(4, 2, 2, e.n)))
+    torch.cuda.synchronize()
+    graphs = []
+    with torch.cuda.stream(streams[2]):
+        e.use_torch_stream()
+        for left, right, c, d, x, packed, w, y in jobs:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=streams[2]):
+                e.ctct_gemm_(d, left, right, g, decay=c)
+                e.ctpt_project_(y, x, packed, g, residual=[x[0], x[1], x[2], x[0]])
+            graphs.append(graph)
+        big = draw(e, 210, g, 260, 2)
+        wide = np.zeros((2, 260, 200), dtype=np.uint32)
+        e.ctpt_project_(e.empty(200, 2, 2, e.n), big, e.gemm_pack_weights(wide, g), g)
+        e.synchronize()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for left, right, c, d, x, packed, w, y in jobs:
+        assert torch.equal(d, want_ctct(e, left, right, g, c))
+        for j in range(4):
+            want = want_project(e, x, w, g, 1, j, None, [x[0], x[1], x[2], x[0]], None)
+            assert torch.equal(y[j, :, 1], want), j
+    del graphs
+    e.close()
+
+
 def test_two_engines_on_two_streams(pkg, params40):
     """Calls of two contexts at once, each with its own tables and workspace."""
     import torch
