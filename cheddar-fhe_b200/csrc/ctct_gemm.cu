@@ -19,15 +19,17 @@
 // bytes come at 2.4, 4.5 and 6.2 TB/s at most (8.9 from L2).
 //
 // m <= 2: bound by reading R, whose words enter one or two results. m >= 3: bound by
-// the 32 x 32 + 64-bit multiply-adds, three instructions each here (20 a clock and
-// SM), so three products a term instead of four:
-//   b a' + a b' = (b + a)(b' + a') - b b' - a a'.
-// Tried instead for m >= 3, with the same result: bytes on the tensor cores
-// (tcgen05.mma wants 64 rows, a position has 2 n; mma.sync with operands split into
-// byte planes and seven 32-bit sums a result, which only fit tensor memory and leave
-// a tile of 4 x 8): 6.1 ms instead of 6.6 for 8 x 64 x 16 on 14 limbs, 6.6 instead of
-// 5.7 for 8 x 16 x 64 on 11. Double precision multiply-adds (56 a clock) need two a
-// product and conversions, as many instructions in all.
+// issue. A 32 x 32 + 64-bit multiply-add is three instructions here, and 64-bit sums
+// of products have to be folded; so a sum T of products is kept twice, as its low 32
+// bits (32-bit multiply-adds) and as a double (rounded), one instruction each on
+// pipes of their own:  T mod q = T - q round(T / q), which only needs the low bits of
+// T and a T / q that is off by less than a quarter. 8 x 64 x 16 on 14 limbs: 6.0
+// ms, 6.6 with 64-bit sums and three products a term (b a' + a b' from the product of
+// sums). Bytes on the tensor cores (tcgen05.mma wants 64 rows, a position has 2 n;
+// mma.sync with operands split into byte planes, whose seven 32-bit sums a result
+// only fit tensor memory and leave a tile of 4 x 8) took 6.1 ms.
+#include <math.h>
+
 #include "context.h"
 #include "kernels.h"
 #include "modmath.cuh"
@@ -179,20 +181,29 @@ __device__ __forceinline__ void store_result(const CtctArgs &a, size_t o, int l,
   to.d2[at] = d2;
 }
 
-// A product of residues is below q^2, a folded sum below q 2^32. For q <= 1.27e9
-// eight products may be added to a folded sum: the high word stays below
-// q + 8 q^2 / 2^32, which is below 2^32 and below 4 q, so subtracting 2 q and q
-// where they fit (two instructions each) folds it again. For larger q every second
-// product is followed by a fold.
-constexpr uint32_t kMaxQ8 = 1270000000u;
+// A 32-bit integer as the double that is the integer times 2^-1074
+__device__ __forceinline__ double tiny(uint32_t v) { return __hiloint2double(0, (int)v); }
 
-template <bool EIGHT>
-__device__ __forceinline__ void fold_sum(uint64_t &s, uint32_t q) {
-  uint32_t hi = (uint32_t)(s >> 32);
-  if constexpr (EIGHT) hi = min(hi, hi - 2 * q);
-  hi = min(hi, hi - q);
-  s = ((uint64_t)hi << 32) | (uint32_t)s;
-}
+// A sum of products of residues: its low 32 bits, and 2^-1074 times the sum, rounded.
+// Up to kSumTerms terms of two products: the sum is below 512 q^2, 512 roundings of
+// 2^-53 of that are 2^18 q 2^-53 < 2^-4 of a quotient by q, and the products with inv
+// and the rounding of inv less than 2^-11.
+constexpr int kSumTerms = 256;
+struct Sum {
+  uint32_t lo;
+  double f;
+  __device__ __forceinline__ void add(uint32_t a, uint32_t b, double b_f) {
+    lo += a * b;
+    f = fma(tiny(a), b_f, f);
+  }
+  // the sum mod q. inv: 2^1000 / q; adding 1.5 2^52 in the scale of the product leaves
+  // the rounded quotient in the low bits
+  __device__ __forceinline__ uint32_t mod(uint32_t q, double inv) const {
+    const double magic = __hiloint2double((1023 + 52 - 74) << 20 | 0x80000, 0);  // 1.5 * 2^(52 - 74)
+    const uint32_t r = lo - (uint32_t)__double2loint(fma(f, inv, magic)) * q;  // in (-q, q)
+    return min(r, r + q);
+  }
+};
 
 // Thread tiles of MT x NT results; WM warps along m, POSITIONS / 32 groups of
 // positions, the other warps along n; stages of TERMS terms
@@ -209,15 +220,10 @@ struct SumsTile {
     return (r < kRowsR ? r : r - kRowsR) >> 1;
   }
 };
-__device__ __forceinline__ void mad_wide(uint64_t &s, uint32_t a, uint32_t b) {
-  asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(s) : "r"(a), "r"(b));
-}
-
-template <int MT, int NT, int WM, int POSITIONS, int TERMS, bool EIGHT>
+template <int MT, int NT, int WM, int POSITIONS, int TERMS>
 __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant__ CtctArgs a,
                                                                  const __grid_constant__ CtctPlan p) {
   using T = SumsTile<MT, NT, WM, POSITIONS, TERMS>;
-  constexpr bool kThree = MT > 2;  // three products a term
   extern __shared__ __align__(16) uint32_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -231,11 +237,12 @@ __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant
     const Where w = where<T>(p, item);
     const int i0 = w.i0 + wi * MT, j0 = w.j0 + wj * NT;
     const uint32_t q = a.q[w.l], nq = a.nqinv[w.l];
-    uint64_t s0[MT][NT], s1[MT][NT], s2[MT][NT];
+    const double inv = a.inv[w.l];
+    Sum s0[MT][NT], s1[MT][NT], s2[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) s0[i][j] = s1[i][j] = s2[i][j] = 0;
+      for (int j = 0; j < NT; j++) s0[i][j] = s1[i][j] = s2[i][j] = {0u, 0.0};
     for (int s = 0; s < feed.n_stages; s++) {
       feed.arrived();  // and all have left the stage before
       feed.step();
@@ -246,43 +253,34 @@ __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant
       for (int u = 0; u < T::kTerms; u++) {
         if (u > 0 && s * T::kTerms + u >= a.k) break;
         const uint32_t *const lp = stage + my_l + u * T::kRowsT * T::C, *const rp = stage + my_r + u * T::kRowsT * T::C;
-        uint32_t lb[MT], la[MT], ls[MT];
+        uint32_t lb[MT], la[MT];
 #pragma unroll
         for (int i = 0; i < MT; i++) {
           lb[i] = lp[2 * i * T::C];
           la[i] = lp[(2 * i + 1) * T::C];
-          if constexpr (kThree) ls[i] = add_mod(lb[i], la[i], q);
         }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
           const uint32_t rb = rp[2 * j * T::C], ra = rp[(2 * j + 1) * T::C];
-          const uint32_t rs = kThree ? add_mod(rb, ra, q) : 0;
+          const double rb_f = rb, ra_f = ra;
 #pragma unroll
           for (int i = 0; i < MT; i++) {
-            mad_wide(s0[i][j], lb[i], rb);
-            if constexpr (kThree) {
-              mad_wide(s1[i][j], ls[i], rs);
-            } else {
-              mad_wide(s1[i][j], lb[i], ra);
-              mad_wide(s1[i][j], la[i], rb);
-              if constexpr (!EIGHT) fold_sum<false>(s1[i][j], q);
-            }
-            mad_wide(s2[i][j], la[i], ra);
+            s0[i][j].add(lb[i], rb, rb_f);
+            s1[i][j].add(lb[i], ra, ra_f);
+            s1[i][j].add(la[i], rb, rb_f);
+            s2[i][j].add(la[i], ra, ra_f);
           }
         }
-        // folds: after two products, or after eight
-        const int done = s * T::kTerms + u;
-        const bool fold = EIGHT ? done % 8 == 7 : done % 2 == 1, fold1 = kThree ? fold : EIGHT && done % 4 == 3;
+      }
+      if ((s + 1) * TERMS % kSumTerms == 0) {
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
-          for (int j = 0; j < NT; j++) {
-            if (fold1) fold_sum<EIGHT>(s1[i][j], q);
-            if (fold) {
-              fold_sum<EIGHT>(s0[i][j], q);
-              fold_sum<EIGHT>(s2[i][j], q);
+          for (int j = 0; j < NT; j++)
+            for (Sum *x : {&s0[i][j], &s1[i][j], &s2[i][j]}) {
+              const uint32_t r = x->mod(q, inv);
+              *x = {r, tiny(r)};
             }
-          }
       }
     }
     const size_t at = (size_t)w.l * kN + w.position + 32 * group + lane;
@@ -291,12 +289,8 @@ __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant
 #pragma unroll
       for (int j = 0; j < NT; j++) {
         if (i0 + i >= a.m || j0 + j >= a.n) continue;
-        fold_sum<EIGHT>(s0[i][j], q);
-        fold_sum<EIGHT>(s1[i][j], q);
-        fold_sum<EIGHT>(s2[i][j], q);
-        const uint32_t d0 = mont_reduce(s0[i][j], q, nq), d2 = mont_reduce(s2[i][j], q, nq);
-        uint32_t d1 = mont_reduce(s1[i][j], q, nq);
-        if constexpr (kThree) d1 = sub_mod(sub_mod(d1, d0, q), d2, q);
+        const uint32_t d0 = mont_reduce(s0[i][j].mod(q, inv), q, nq), d1 = mont_reduce(s1[i][j].mod(q, inv), q, nq),
+                       d2 = mont_reduce(s2[i][j].mod(q, inv), q, nq);
         store_result(a, (size_t)(i0 + i) * a.n + j0 + j, w.l, at, d0, d1, d2, q, nq);
       }
   }
@@ -320,31 +314,32 @@ int launch_tiles(const Context &ctx, const CtctArgs &a, Kernel kernel, PerDevice
   return 0;
 }
 
-template <int MT, int NT, int WM, int POSITIONS, int TERMS, bool EIGHT>
+template <int MT, int NT, int WM, int POSITIONS, int TERMS>
 int launch_sums(const Context &ctx, const CtctArgs &a) {
   using T = SumsTile<MT, NT, WM, POSITIONS, TERMS>;
   static_assert(T::kStages >= 3, "copies ahead of the products");
   static PerDeviceOnce once;
-  return launch_tiles<T>(ctx, a, ctct_sums_kernel<MT, NT, WM, POSITIONS, TERMS, EIGHT>, once);
-}
-
-// Tiles of m x 32 (m <= 2), 4 x 16 or 8 x 8 results on 64 positions; few columns
-// leave warps for more positions.
-template <bool EIGHT>
-int launch(const Context &ctx, const CtctArgs &a) {
-  if (a.m == 1) return a.n > 8 ? launch_sums<1, 4, 1, 64, 2, EIGHT>(ctx, a) : launch_sums<1, 4, 1, 256, 2, EIGHT>(ctx, a);
-  if (a.m == 2) return a.n > 8 ? launch_sums<2, 4, 1, 64, 2, EIGHT>(ctx, a) : launch_sums<2, 4, 1, 256, 2, EIGHT>(ctx, a);
-  if (a.m <= 4) return a.n > 8 ? launch_sums<4, 2, 1, 64, 4, EIGHT>(ctx, a) : launch_sums<4, 2, 1, 128, 4, EIGHT>(ctx, a);
-  return launch_sums<4, 2, 2, 64, 8, EIGHT>(ctx, a);
+  return launch_tiles<T>(ctx, a, ctct_sums_kernel<MT, NT, WM, POSITIONS, TERMS>, once);
 }
 
 }  // namespace
 
-// args.m <= args.n
+// args.m <= args.n. Tiles of m x 32 (m <= 2), 4 x 16 or 8 x 8 results on 64 positions;
+// few columns leave warps for more positions.
 int launch_ctct_gemm(const Context &ctx, const CtctArgs &args) {
-  uint32_t top = 0;
-  for (int l = 0; l < args.n_limbs; l++) top = max(top, args.q[l]);
-  if (int r = top <= kMaxQ8 ? launch<true>(ctx, args) : launch<false>(ctx, args)) return r;
+  CtctArgs a = args;
+  for (int l = 0; l < a.n_limbs; l++) a.inv[l] = ldexp(1.0 / a.q[l], 1000);
+  const bool wide = a.n > 8;
+  int r;
+  if (a.m == 1)
+    r = wide ? launch_sums<1, 4, 1, 64, 2>(ctx, a) : launch_sums<1, 4, 1, 256, 2>(ctx, a);
+  else if (a.m == 2)
+    r = wide ? launch_sums<2, 4, 1, 64, 2>(ctx, a) : launch_sums<2, 4, 1, 256, 2>(ctx, a);
+  else if (a.m <= 4)
+    r = wide ? launch_sums<4, 2, 1, 64, 4>(ctx, a) : launch_sums<4, 2, 1, 128, 4>(ctx, a);
+  else
+    r = launch_sums<4, 2, 2, 64, 8>(ctx, a);
+  if (r) return r;
   CFHE_CUDA(cudaGetLastError());
   return 0;
 }

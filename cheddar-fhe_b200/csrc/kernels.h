@@ -225,6 +225,7 @@ struct CtctArgs {
   const CtctOut *out;
   const uint32_t *consts;  // constant weights [m * n][n_limbs] on the device, or null
   uint32_t q[kMaxLimbs], nqinv[kMaxLimbs];
+  double inv[kMaxLimbs];   // 2^1000 / q, filled by the launcher
 };
 int launch_ctct_gemm(const Context &ctx, const CtctArgs &args);
 // sampling.cu: client-side sampling and encryption
