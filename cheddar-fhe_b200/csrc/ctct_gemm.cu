@@ -19,15 +19,19 @@
 // bytes come at 2.4, 4.5 and 6.2 TB/s at most (8.9 from L2).
 //
 // m <= 2: bound by reading R, whose words enter one or two results. m >= 3: bound by
-// issue. A 32 x 32 + 64-bit multiply-add is three instructions here, and 64-bit sums
-// of products have to be folded; so a sum T of products is kept twice, as its low 32
-// bits (32-bit multiply-adds) and as a double (rounded), one instruction each on
-// pipes of their own:  T mod q = T - q round(T / q), which only needs the low bits of
-// T and a T / q that is off by less than a quarter. 8 x 64 x 16 on 14 limbs: 6.0
-// ms, 6.6 with 64-bit sums and three products a term (b a' + a b' from the product of
-// sums). Bytes on the tensor cores (tcgen05.mma wants 64 rows, a position has 2 n;
-// mma.sync with operands split into byte planes, whose seven 32-bit sums a result
-// only fit tensor memory and leave a tile of 4 x 8) took 6.1 ms.
+// the multipliers. A 32 x 32 + 64-bit multiply-add is three instructions here, and
+// 64-bit sums of products have to be folded; so a sum T of products is kept twice, as
+// its low 32 bits (32-bit multiply-adds) and as a double (rounded), one instruction
+// each:  T mod q = T - q round(T / q), which only needs the low bits of T and a T / q
+// that is off by less than a quarter. Three products a term: b a' + a b' comes from the
+// product of the sums. The two kinds of multiply-add hardly overlap (24 of each for
+// four warps: 270 and 387 clocks alone, 590 to 710 together), which is 3.8 of the 5.3
+// ms of 8 x 64 x 16 on 14 limbs. With 64-bit sums it took 6.6 ms, with four products a
+// term and each result's weight fetched on its own 6.0; bytes on the tensor cores
+// (tcgen05.mma wants 64 rows, a position has 2 n; mma.sync with operands split into byte
+// planes, whose seven 32-bit sums a result only fit tensor memory and leave a tile of
+// 4 x 8) 6.1; copies of whole rows that the warps wait for one by one, so that they may
+// be stages apart, 6.6.
 #include <math.h>
 
 #include "context.h"
@@ -166,28 +170,14 @@ struct Feed {
   }
 };
 
-// The words of result o: weighted, stored
-__device__ __forceinline__ void store_result(const CtctArgs &a, size_t o, int l, size_t at, uint32_t d0, uint32_t d1,
-                                             uint32_t d2, uint32_t q, uint32_t nq) {
-  const CtctOut to = a.out[o];
-  if (to.weight || a.consts) {
-    const uint32_t v = to.weight ? to.weight[at] : a.consts[o * a.n_limbs + l];
-    d0 = mont_mul(d0, v, q, nq);
-    d1 = mont_mul(d1, v, q, nq);
-    d2 = mont_mul(d2, v, q, nq);
-  }
-  to.d0[at] = d0;
-  to.d1[at] = d1;
-  to.d2[at] = d2;
-}
-
 // A 32-bit integer as the double that is the integer times 2^-1074
 __device__ __forceinline__ double tiny(uint32_t v) { return __hiloint2double(0, (int)v); }
 
 // A sum of products of residues: its low 32 bits, and 2^-1074 times the sum, rounded.
-// Up to kSumTerms terms of two products: the sum is below 512 q^2, 512 roundings of
-// 2^-53 of that are 2^18 q 2^-53 < 2^-4 of a quotient by q, and the products with inv
-// and the rounding of inv less than 2^-11.
+// Up to kSumTerms terms of two products, or of one of sums of two residues: the sum is
+// below 1024 q^2, its roundings together (512 of sums below 512 q^2, 256 of sums below
+// 1024 q^2) less than 2^18 q^2 2^-53, that is 2^-4 of a quotient by q, and the product
+// with inv and the rounding of inv less than 2^-11.
 constexpr int kSumTerms = 256;
 struct Sum {
   uint32_t lo;
@@ -222,8 +212,9 @@ struct SumsTile {
 };
 template <int MT, int NT, int WM, int POSITIONS, int TERMS>
 __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant__ CtctArgs a,
-                                                                 const __grid_constant__ CtctPlan p) {
+                                                           const __grid_constant__ CtctPlan p) {
   using T = SumsTile<MT, NT, WM, POSITIONS, TERMS>;
+  constexpr bool kThree = MT > 2;  // three products a term
   extern __shared__ __align__(16) uint32_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -253,21 +244,26 @@ __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant
       for (int u = 0; u < T::kTerms; u++) {
         if (u > 0 && s * T::kTerms + u >= a.k) break;
         const uint32_t *const lp = stage + my_l + u * T::kRowsT * T::C, *const rp = stage + my_r + u * T::kRowsT * T::C;
-        uint32_t lb[MT], la[MT];
+        uint32_t lb[MT], la[MT], ls[MT];
 #pragma unroll
         for (int i = 0; i < MT; i++) {
           lb[i] = lp[2 * i * T::C];
           la[i] = lp[(2 * i + 1) * T::C];
+          ls[i] = lb[i] + la[i];
         }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          const uint32_t rb = rp[2 * j * T::C], ra = rp[(2 * j + 1) * T::C];
-          const double rb_f = rb, ra_f = ra;
+          const uint32_t rb = rp[2 * j * T::C], ra = rp[(2 * j + 1) * T::C], rs = rb + ra;
+          const double rb_f = rb, ra_f = ra, rs_f = rb_f + ra_f;
 #pragma unroll
           for (int i = 0; i < MT; i++) {
             s0[i][j].add(lb[i], rb, rb_f);
-            s1[i][j].add(lb[i], ra, ra_f);
-            s1[i][j].add(la[i], rb, rb_f);
+            if (kThree) {
+              s1[i][j].add(ls[i], rs, rs_f);
+            } else {
+              s1[i][j].add(lb[i], ra, ra_f);
+              s1[i][j].add(la[i], rb, rb_f);
+            }
             s2[i][j].add(la[i], ra, ra_f);
           }
         }
@@ -283,15 +279,52 @@ __global__ void __launch_bounds__(512, 1) ctct_sums_kernel(const __grid_constant
             }
       }
     }
+    // The weights are on their way before the first is waited for, the pointers of a
+    // result before the one before it is stored.
     const size_t at = (size_t)w.l * kN + w.position + 32 * group + lane;
+    if (i0 >= a.m || j0 >= a.n) continue;
+    const size_t o0 = (size_t)i0 * a.n + j0;
+    auto there = [&](int i, int j) { return i0 + i < a.m && j0 + j < a.n; };
+    uint32_t v[MT][NT];
+    const uint32_t *weight[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) weight[i][j] = there(i, j) ? a.out[o0 + i * a.n + j].weight : nullptr;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+        v[i][j] = weight[i][j]                 ? weight[i][j][at]
+                  : a.consts && there(i, j) ? a.consts[(o0 + i * a.n + j) * a.n_limbs + w.l]
+                                            : 0;
+    CtctOut next = a.out[o0];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
       for (int j = 0; j < NT; j++) {
-        if (i0 + i >= a.m || j0 + j >= a.n) continue;
-        const uint32_t d0 = mont_reduce(s0[i][j].mod(q, inv), q, nq), d1 = mont_reduce(s1[i][j].mod(q, inv), q, nq),
-                       d2 = mont_reduce(s2[i][j].mod(q, inv), q, nq);
-        store_result(a, (size_t)(i0 + i) * a.n + j0 + j, w.l, at, d0, d1, d2, q, nq);
+        const CtctOut to = next;
+        const int ni = j + 1 < NT ? i : i + 1, nj = j + 1 < NT ? j + 1 : 0;
+        if (ni < MT && there(ni, nj)) next = a.out[o0 + ni * a.n + nj];
+        const uint32_t t0 = s0[i][j].mod(q, inv), t2 = s2[i][j].mod(q, inv);
+        uint32_t t1 = s1[i][j].mod(q, inv);
+        if (kThree) {
+          t1 -= t0;
+          t1 = min(t1, t1 + q);
+          t1 -= t2;
+          t1 = min(t1, t1 + q);
+        }
+        uint32_t d0 = mont_reduce(t0, q, nq), d1 = mont_reduce(t1, q, nq), d2 = mont_reduce(t2, q, nq);
+        if (to.weight || a.consts) {
+          d0 = mont_mul(d0, v[i][j], q, nq);
+          d1 = mont_mul(d1, v[i][j], q, nq);
+          d2 = mont_mul(d2, v[i][j], q, nq);
+        }
+        if (there(i, j)) {
+          to.d0[at] = d0;
+          to.d1[at] = d1;
+          to.d2[at] = d2;
+        }
       }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
