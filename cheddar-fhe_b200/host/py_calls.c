@@ -266,14 +266,21 @@ done:
   return ok ? 0 : -1;
 }
 
-/* lead: 1 (a list of ciphertexts) or 2 (a matrix); holes: a list may hold None */
-static int get_cts(PyObject *o, int lead, int parts, int holes, const ct_shape *want, ct_table *t) {
+/* lead: 1 (a list of ciphertexts) or 2 (a matrix); holes: a list may hold None.
+ * Polynomials closer than their size (an expanded tensor) overlap: inputs may. */
+enum { INPUT, INPUT_WITH_HOLES, OUTPUT };
+static int get_cts(PyObject *o, int lead, int parts, int kind, const ct_shape *want, ct_table *t) {
   long long dim[5], stride[5];
   char *base;
   t->p = NULL;
   const int each = parts ? parts : 1;
   if (!PyList_Check(o) && !PyTuple_Check(o)) {
     if (get_layout(o, lead, parts, want, &base, dim, stride)) return -1;
+    for (int i = 0; kind == OUTPUT && i < lead + (parts ? 1 : 0); i++)
+      if (dim[i] > 1 && llabs(stride[i]) < want->limbs * want->n) {
+        PyErr_SetString(PyExc_ValueError, "the polynomials of an output overlap");
+        return -1;
+      }
     const long long cols = lead == 2 ? dim[1] : 1, cs = lead == 2 ? stride[1] : 0;
     if (new_cts(t, dim[0], cols, parts)) return -1;
     for (int p = 0; p < each; p++)
@@ -302,7 +309,7 @@ static int get_cts(PyObject *o, int lead, int parts, int holes, const ct_shape *
     }
     for (Py_ssize_t c = 0; c < cols; c++) {
       PyObject *x = lead == 2 ? PySequence_Fast_GET_ITEM(row, c) : row;
-      if (holes && x == Py_None) continue;
+      if (kind == INPUT_WITH_HOLES && x == Py_None) continue;
       if (get_layout(x, 0, parts, want, &base, dim, stride)) {
         free_cts(t);
         return -1;
@@ -731,13 +738,23 @@ static PyObject *py_ctpt_project(PyObject *self, PyObject *const *a, Py_ssize_t 
   ct_shape want;
   void *w;
   int rc;
-  PyObject *ret = NULL;
-  if (get_ll(a[1], &want.device) || get_ptr(a[4], &w) || get_ints(a[5], 'i', &g)) return NULL;
+  long long device;
+  PyObject *ret = NULL, *e = PyObject_CallMethodNoArgs(a[4], s_get_device);
+  if (!e || get_ll(e, &device) || get_ll(a[1], &want.device) || get_ptr(a[4], &w)) {
+    Py_XDECREF(e);
+    return NULL;
+  }
+  Py_DECREF(e);
+  if (device != want.device) {
+    PyErr_SetString(PyExc_ValueError, "the packed weights are not on the engine's device");
+    return NULL;
+  }
+  if (get_ints(a[5], 'i', &g)) return NULL;
   want.limbs = g.n;
   want.n = cfhe_degree(HANDLE(a[0]));
-  if (get_cts(a[2], 1, 2, 0, &want, &y) || get_cts(a[3], 1, 2, 0, &want, &x)) goto done;
+  if (get_cts(a[2], 1, 2, OUTPUT, &want, &y) || get_cts(a[3], 1, 2, INPUT, &want, &x)) goto done;
   if (a[7] != Py_None) {
-    if (get_cts(a[7], 1, 2, 1, &want, &r)) goto done;
+    if (get_cts(a[7], 1, 2, INPUT_WITH_HOLES, &want, &r)) goto done;
     if (r.rows != y.rows) {
       PyErr_SetString(PyExc_ValueError, "one residual per output is expected");
       goto done;
@@ -773,7 +790,7 @@ static PyObject *py_rotary(PyObject *self, PyObject *const *a, Py_ssize_t n) {
   if (get_ll(a[1], &want.device) || get_converted(a[7], &halves) || get_ints(a[6], 'i', &g)) return NULL;
   want.limbs = g.n;
   want.n = cfhe_degree(HANDLE(a[0]));
-  if (get_cts(a[2], 2, 2, 0, &want, &y) || get_cts(a[3], 2, 2, 0, &want, &x)) goto done;
+  if (get_cts(a[2], 2, 2, OUTPUT, &want, &y) || get_cts(a[3], 2, 2, INPUT, &want, &x)) goto done;
   if (y.rows != x.rows || y.cols != x.cols || x.cols % 2) {
     PyErr_SetString(PyExc_ValueError, "inputs and outputs of the same even number of features are expected");
     goto done;
@@ -785,7 +802,7 @@ static PyObject *py_rotary(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     if (get_words(a[4], pairs * want.limbs, &cw) || get_words(a[5], pairs * want.limbs, &sw)) goto done;
     ENTER(cfhe_rotary_token(HANDLE(a[0]), yp, xp, (int)(2 * x.rows), (int)pairs, halves != 0, cw.p, sw.p, g.p, g.n));
   } else {
-    if (get_cts(a[4], 1, 0, 0, &want, &c) || get_cts(a[5], 1, 0, 0, &want, &s)) goto done;
+    if (get_cts(a[4], 1, 0, INPUT, &want, &c) || get_cts(a[5], 1, 0, INPUT, &want, &s)) goto done;
     if (c.rows != pairs || s.rows != pairs) {
       PyErr_SetString(PyExc_ValueError, "one cosine and one sine per pair of features are expected");
       goto done;
@@ -818,7 +835,8 @@ static PyObject *py_ctct_gemm(PyObject *self, PyObject *const *a, Py_ssize_t n) 
   if (get_ll(a[1], &want.device) || get_ints(a[5], 'i', &g)) return NULL;
   want.limbs = g.n;
   want.n = cfhe_degree(HANDLE(a[0]));
-  if (get_cts(a[2], 2, 3, 0, &want, &d) || get_cts(a[3], 2, 2, 0, &want, &l) || get_cts(a[4], 2, 2, 0, &want, &r))
+  if (get_cts(a[2], 2, 3, OUTPUT, &want, &d) || get_cts(a[3], 2, 2, INPUT, &want, &l) ||
+      get_cts(a[4], 2, 2, INPUT, &want, &r))
     goto done;
   if (l.rows != d.rows || r.cols != d.cols || l.cols != r.rows) {
     PyErr_SetString(PyExc_ValueError, "the sizes of the matrices do not fit");
@@ -829,7 +847,7 @@ static PyObject *py_ctct_gemm(PyObject *self, PyObject *const *a, Py_ssize_t n) 
     if (PyObject_CheckBuffer(a[6])) {
       if (get_words(a[6], mn * want.limbs, &ww)) goto done;
     } else {
-      if (get_cts(a[6], 2, 0, 0, &want, &w)) goto done;
+      if (get_cts(a[6], 2, 0, INPUT, &want, &w)) goto done;
       if (w.rows != d.rows || w.cols != d.cols) {
         PyErr_SetString(PyExc_ValueError, "one decay per result is expected");
         goto done;

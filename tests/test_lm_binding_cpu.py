@@ -180,3 +180,27 @@ def test_refusals(b):
     b.refused(ValueError, k.ctct_gemm, 0, 0, d, left, right, G, Tensor(1, 1, 2, 2, N))
     b.refused(ValueError, k.ctct_gemm, 0, 0, d, [[Tensor(1, 2, 2, N)] * 2, [Tensor(1, 2, 2, N)]], right, G, None)
     b.refused(TypeError, k.ctct_gemm, 0, 0, d, [Tensor(1, 2, 2, N)] * 2, right, G, None)
+
+
+def test_outputs_that_overlap_are_refused(b):
+    """An expanded tensor as output has one polynomial in several places; inputs may."""
+    k, w, x = b.k, Tensor(16, 4), Tensor(1, 3, 2, 2, N, stride=(0, 2 * N, N, 1))
+    assert k.ctpt_project(0, 0, Tensor(1, 3, 2, 2, N), x, w, G, None, x, None) == 0
+    b.refused(ValueError, k.ctpt_project, 0, 0, x, x, w, G, None, None, None)
+    b.refused(ValueError, k.ctpt_project, 0, 0, Tensor(1, 3, 2, 2, N, stride=(4 * N, 0, N, 1)), x, w, G, None, None, None)
+    words = np.zeros(4, dtype=np.uint32)
+    y = Tensor(1, 2, 4, 2, 2, N, stride=(4 * N, 0, 2 * N, N, 1))
+    b.refused(ValueError, k.rotary, 0, 0, y, Tensor(1, 2, 4, 2, 2, N), words, words, G, False)
+    left, right = Tensor(1, 2, 2, 2, 2, N, stride=(0, 4 * N, 2 * N, N, 1)), Tensor(1, 2, 3, 2, 2, N)
+    assert k.ctct_gemm(0, 0, Tensor(1, 2, 3, 3, 2, N), left, right, G, None) == 0
+    b.refused(ValueError, k.ctct_gemm, 0, 0, Tensor(1, 2, 3, 3, 2, N, stride=(N, 6 * N, 2 * N, N, 1)), left, right, G, None)
+    one = Tensor(1, 1, 3, 2, 2, N, stride=(0, 4 * N, 2 * N, N, 1))  # a single row's stride means nothing
+    assert k.rotary(0, 0, Tensor(1, 1, 4, 2, 2, N, stride=(0, 4 * N, 2 * N, N, 1)), Tensor(1, 1, 4, 2, 2, N), words, words,
+                    G, False) == 0
+    b.refused(ValueError, k.ctct_gemm, 0, 0, one, left, right, G, None)
+
+
+def test_packed_weights_of_another_device_are_refused(b):
+    y, x = Tensor(1, 3, 2, 2, N), Tensor(1, 2, 2, 2, N)
+    for device in (-1, 1):
+        b.refused(ValueError, b.k.ctpt_project, 0, 0, y, x, Tensor(16, 4, device=device), G, None, None, None)

@@ -241,8 +241,8 @@ def primes_below(bound, count):
 
 @pytest.mark.parametrize("bound", [1270000000, 1 << 31])
 def test_operators_at_the_largest_primes(pkg, bound):
-    """The largest prime with eight products between two folds of a sum, and the
-    largest there are (two): largest words, then random ones, in every kernel."""
+    """Primes of the shipped size and the largest there are: largest words, then random
+    ones, in every kernel."""
     main = primes_below(bound, 4)
     aux = primes_below(1 << 29, 2)
     e = pkg.Engine({"log_degree": 16, "main_primes": main, "terminal_primes": [], "auxiliary_primes": aux,
@@ -281,6 +281,30 @@ def test_operators_at_the_largest_primes(pkg, bound):
     for j in range(5):
         for l in range(2):
             assert e.torch.equal(y[j, :, l], want_project(e, x[0], w, g, l, j, b, r, s)), (j, l)
+    e.close()
+
+
+@pytest.mark.parametrize("m,n", [(1, 3), (1, 10), (2, 5), (2, 9), (4, 4), (3, 11), (6, 7)])
+def test_ctct_gemm_long_sums(pkg, m, n):
+    """More terms than a sum takes before it is brought back below its bound, at the
+    largest primes: one ciphertext in all places of a matrix, so that a result is k
+    times their product."""
+    bound = 1 << 31
+    e = pkg.Engine({"log_degree": 16, "main_primes": primes_below(bound, 2), "terminal_primes": [],
+                    "auxiliary_primes": primes_below(1 << 29, 2), "level_config": [[1, 0], [2, 0]],
+                    "additional_base": [0, 0]})
+    g = [0, 1]
+    x, y = draw(e, 220, g, 1, 1, 2), draw(e, 221, g, 1, 1, 2)
+    for l in range(2):
+        x[..., l, :128] = int(e.primes[l]) - 1
+        y[..., l, :128] = int(e.primes[l]) - 1
+    one = want_ctct(e, x, y, g, None).long()
+    for k in (255, 256, 257, 511, 513, 1030):
+        d = e.empty(m, n, 3, 2, e.n).fill_(-1)
+        e.ctct_gemm_(d, x.expand(m, k, 2, 2, e.n), y.expand(k, n, 2, 2, e.n), g)
+        for l in range(2):
+            want = one[:, :, :, l] * k % int(e.primes[l])
+            assert e.torch.equal(d[:, :, :, l].long(), want.expand(m, n, 3, e.n)), (k, l)
     e.close()
 
 
