@@ -266,7 +266,11 @@ CFHE_API int cfhe_rotary_token(cfhe_context *ctx, uint32_t *const *y, const uint
  * at most one of the two. m, k, n from 1 to 8192, at most 65535 results and 2^20
  * operands; outputs overlap nothing; polynomials on 16-byte boundaries. Same
  * words as cfhe_tensor_accum per result, then cfhe_binary / cfhe_const_op
- * (multiply) on its three parts. */
+ * (multiply) on its three parts.
+ * The four calls above read their HOST tables before they return and may be captured
+ * into a graph; a captured projection or product keeps device memory of its own for
+ * tables and temporaries until the context is destroyed, which has to outlive the
+ * graph. */
 CFHE_API int cfhe_ctct_gemm(cfhe_context *ctx, uint32_t *const *d0, uint32_t *const *d1, uint32_t *const *d2,
                             const uint32_t *const *lb, const uint32_t *const *la, const uint32_t *const *rb,
                             const uint32_t *const *ra, int m, int k, int n, const uint32_t *const *decay_pt,
