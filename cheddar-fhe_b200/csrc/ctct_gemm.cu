@@ -357,19 +357,25 @@ int launch_sums(const Context &ctx, const CtctArgs &a) {
 
 }  // namespace
 
-// args.m <= args.n. Tiles of m x 32 (m <= 2), 4 x 16 or 8 x 8 results on 64 positions;
-// few columns leave warps for more positions.
+// args.m <= args.n. Tiles of 8 columns (4 where there are no more, so that no warp is
+// without results) and as many positions as the warps then have room for: longer rows
+// and no columns without results are worth more than reading L once per 8 columns
+// instead of once per 32. Rows of 1 KB and 8 columns against 256 bytes and 32, on 7
+// limbs: 1 x 60 x 64 1910 -> 1924 us, 1 x 16 x 17 244 -> 199, 2 x 64 x 33 2688 -> 1610;
+// 4 x 16 x 64 (512 bytes against 256, 16 columns) 1379 -> 1397, 3 x 16 x 17 689 -> 447;
+// 4 columns against 8: 2 x 5 x 3 47 -> 39, 4 x 64 x 4 406 -> 338. With m >= 5 L is half of the
+// rows: 8 x 64 x 8 947 us, with 512 bytes and 4 columns 1150.
 int launch_ctct_gemm(const Context &ctx, const CtctArgs &args) {
   CtctArgs a = args;
   for (int l = 0; l < a.n_limbs; l++) a.inv[l] = ldexp(1.0 / a.q[l], 1000);
-  const bool wide = a.n > 8;
+  const bool narrow = a.n <= 4;
   int r;
   if (a.m == 1)
-    r = wide ? launch_sums<1, 4, 1, 64, 2>(ctx, a) : launch_sums<1, 4, 1, 256, 2>(ctx, a);
+    r = narrow ? launch_sums<1, 2, 1, 256, 4>(ctx, a) : launch_sums<1, 4, 1, 256, 2>(ctx, a);
   else if (a.m == 2)
-    r = wide ? launch_sums<2, 4, 1, 64, 2>(ctx, a) : launch_sums<2, 4, 1, 256, 2>(ctx, a);
+    r = narrow ? launch_sums<2, 2, 1, 256, 4>(ctx, a) : launch_sums<2, 4, 1, 256, 2>(ctx, a);
   else if (a.m <= 4)
-    r = wide ? launch_sums<4, 2, 1, 64, 4>(ctx, a) : launch_sums<4, 2, 1, 128, 4>(ctx, a);
+    r = narrow ? launch_sums<4, 2, 1, 256, 2>(ctx, a) : launch_sums<4, 2, 1, 128, 4>(ctx, a);
   else
     r = launch_sums<4, 2, 2, 64, 8>(ctx, a);
   if (r) return r;

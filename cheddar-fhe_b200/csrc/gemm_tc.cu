@@ -601,12 +601,13 @@ int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const
 // polynomials of a limb find its weights in L2.
 //
 // From three output tiles on an entry's activations are packed inside the products
-// of the entry before (two buffers); with fewer, entries go in groups of up to 64 MiB
-// of packed activations, two launches a group (packing inside the products was slower:
-// 130 x 77 on 9 limbs 1.00 instead of 0.78 ms).
+// of the entry before (two buffers); with fewer, entries go in groups of up to 96 MiB
+// of packed activations (they and a group's results stay in L2), two launches a group (packing inside the products was slower:
+// 130 x 77 on 9 limbs 1.00 instead of 0.78 ms; now 0.70 ms in groups of one, 0.67 of two,
+// 0.66 of four).
 int project_buffers(int n_in, int n_out, int n_limbs) {
   if (gemm_packs_ahead(n_out, 2 * n_limbs)) return 2;
-  const size_t fit = ((size_t)64 << 20) / gemm_scratch_bytes(n_in);
+  const size_t fit = ((size_t)96 << 20) / gemm_scratch_bytes(n_in);
   return (int)std::min({(size_t)kMaxGroup, (size_t)2 * n_limbs, std::max(fit, (size_t)1)});
 }
 
