@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
 // residual a word takes some 35 instructions, so few inputs (32: two K steps a tile)
 // leave the epilogue the longer part. Against a CTA a tile: 32 x 64 on 3 limbs
 // 95 -> 82 us, 130 x 77 with a residual on 9 limbs 770 -> 690 us; 768 x 768 on 11
-// limbs takes 12.2 to 13.1 ms either way, at the power limit.
+// limbs takes 12.2 to 13.1 ms either way, at the power limit. (With the failure flag
+// read at the top of a tile and larger groups 76 and 654 us.)
 constexpr int kPjWarps = 8, kPjThreads = 32 * (kPjWarps + 2), kPjOuts = kGmOutTile / 2;
 
 __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_constant__ GemmArgs a,
@@ -424,7 +425,15 @@ __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_
         s_res[b][tid] = e.res && j < a.n_out ? e.res[j] : nullptr;
         s_bias[b][tid] = e.bias && j < a.n_out ? e.bias[j] : 0;
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * kPjWarps) : "memory");
+      // the tables are there; all of these warps go on, or none where a wait ran out
+      uint32_t failed = *(volatile int *)&s_failed;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbar.red.or.pred q, 1, %1, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "+r"(failed)
+          : "n"(32 * kPjWarps)
+          : "memory");
+      if (failed) break;
       // meanwhile: this tile's share of the next entry's packing (one entry a launch then)
       if (a.xp_next) {
         const long long units = (long long)kTilesM * 4 * a.k_steps;
@@ -443,8 +452,10 @@ __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_
       }
       const bool arrived = mbar_wait(smem_u32(accum), n & 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (!arrived) fail();
-      if (!arrived || *(volatile int *)&s_failed) break;
+      if (!__all_sync(~0u, arrived)) {
+        fail();
+        continue;
+      }
       const uint32_t q = e.q, nq = e.nqinv, res_scale = e.res_scale;
 #pragma unroll
       for (int j0 = 0; j0 < kPjOuts; j0 += 8) {
@@ -603,8 +614,8 @@ int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const
 // From three output tiles on an entry's activations are packed inside the products
 // of the entry before (two buffers); with fewer, entries go in groups of up to 96 MiB
 // of packed activations (they and a group's results stay in L2), two launches a group (packing inside the products was slower:
-// 130 x 77 on 9 limbs 1.00 instead of 0.78 ms; now 0.70 ms in groups of one, 0.67 of two,
-// 0.66 of four).
+// 130 x 77 on 9 limbs 1.00 instead of 0.78 ms; 0.70 ms in groups of one, 0.67 of two, 0.66 of
+// four).
 int project_buffers(int n_in, int n_out, int n_limbs) {
   if (gemm_packs_ahead(n_out, 2 * n_limbs)) return 2;
   const size_t fit = ((size_t)96 << 20) / gemm_scratch_bytes(n_in);
