@@ -1,5 +1,5 @@
 // TEST INFRASTRUCTURE: float64 restatement of a transformer layer with decayed
-// linear attention and rotary positions on several axes, used only as the checker of
+// linear attention and rotary positions on several axes, used only as the oracle of
 // the encrypted layer in tests. Parity unpinned by the reference, which has no
 // transformer code; stated in natural units from the definitions, with the exact or
 // the Chebyshev form of the remaining non-linear functions (transformer_plain.h).

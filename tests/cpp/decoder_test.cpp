@@ -93,7 +93,7 @@ static void Tokens(std::shared_ptr<BootContext<word>> ctx, UserInterface<word> &
       plain_decoder::Turn(x[0], p, t + 1, 1, D);
       plain_decoder::Turn(x[1], p, t + 1, 1, D);
       const auto want = plain_decoder::Attention(x[0], x[1], x[2], {decay}, t + 1, D);
-      for (int d = 0; d < D; d++)  // without the checker's 1 / sqrt(D)
+      for (int d = 0; d < D; d++)  // without the oracle's 1 / sqrt(D)
         worst = std::max(worst, std::abs(got[d][i].real() - 2.0 * want[(size_t)t * D + d]));
     }
   }
