@@ -36,7 +36,8 @@
 // epilogue. Two CTAs share an SM (2 x 256 tensor-memory columns).
 //
 // Every barrier wait is bounded; a wait that runs out raises the context's
-// error flag and the CTA winds down without touching the accumulators.
+// error flag and the CTA winds down: no result is stored after the flag of its own
+// failure is up, and it leaves only when the copies that it started have landed.
 #include <algorithm>
 #include <vector>
 
@@ -59,6 +60,12 @@ constexpr int kGmThreads = 192;     // warps 0-3 epilogue, warp 4 copies, warp 5
 constexpr int kGmSmem = kGmStages * (kGmAStage + kGmBStage) + 128;  // and the barriers
 constexpr uint32_t kWaitHintNs = 2000;
 constexpr uint32_t kSpinLimit = 1u << 20;
+// of the wait for a stage's operands; a test makes it run out
+#ifdef CFHE_STAGE_TRIES
+constexpr uint32_t kStageTries = CFHE_STAGE_TRIES;
+#else
+constexpr uint32_t kStageTries = kSpinLimit;
+#endif
 
 struct GemmArgs {
   const uint8_t *xp;          // packed activations of this limb: [N/128][K/16][2048]
@@ -123,10 +130,27 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 // false: the wait ran out
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kSpinLimit; i++)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t tries = kSpinLimit) {
+  for (uint32_t i = 0; i < tries; i++)
     if (mbar_try_wait(bar, parity)) return true;
   return false;
+}
+// A wait of this CTA ran out. The thread's own commits come behind the flag.
+__device__ __forceinline__ void give_up(int *error_flag, int *failed) {
+  atomicExch(error_flag, 1);
+  atomicExch(failed, 1);
+  __threadfence_block();
+}
+// What the copying thread started, up to stage `s` of `round` (not filled any more),
+// has landed. Where the MMAs wait for them all, that costs nothing; where
+// they gave up, a copy still on its way would write into another CTA's shared memory.
+__device__ __forceinline__ bool copies_landed(const uint64_t *full, int s, int round) {
+  bool ok = true;
+  for (int i = 0; i < kGmStages; i++) {
+    const int last = i < s ? round : round - 1;  // the round that stage i was last filled in
+    if (last >= 0 && !mbar_wait(smem_u32(full + i), last & 1)) ok = false;
+  }
+  return ok;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -242,24 +266,24 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
     // ---- copies: stage s receives K step ks when the MMAs of step ks - kGmStages have left it
     const uint8_t *ap = a.xp + (size_t)m_tile * a.k_steps * kGmAStage;
     const uint8_t *bp = a.wp + (size_t)n_tile * a.k_steps * kGmBStage;
-    for (int ks = 0; ks < a.k_steps; ks++) {
+    int ks = 0;
+    for (; ks < a.k_steps; ks++) {
       const int s = ks % kGmStages, round = ks / kGmStages;
       if (round > 0 && !mbar_wait(smem_u32(empty + s), (round - 1) & 1)) {
-        atomicExch(a.error_flag, 1);
-        atomicExch(&s_failed, 1);
+        give_up(a.error_flag, &s_failed);
         break;
       }
       mbar_expect_tx(smem_u32(full + s), kGmAStage + kGmBStage);
       bulk_load(smem_u32(sA + s * kGmAStage), ap + (size_t)ks * kGmAStage, kGmAStage, smem_u32(full + s));
       bulk_load(smem_u32(sB + s * kGmBStage), bp + (size_t)ks * kGmBStage, kGmBStage, smem_u32(full + s));
     }
+    if (!copies_landed(full, ks % kGmStages, ks / kGmStages)) give_up(a.error_flag, &s_failed);
   } else if (tid == 5 * 32) {
     // ---- MMAs
     for (int ks = 0; ks < a.k_steps; ks++) {
       const int s = ks % kGmStages, round = ks / kGmStages;
-      if (!mbar_wait(smem_u32(full + s), round & 1)) {
-        atomicExch(a.error_flag, 1);
-        atomicExch(&s_failed, 1);
+      if (!mbar_wait(smem_u32(full + s), round & 1, kStageTries)) {
+        give_up(a.error_flag, &s_failed);
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -356,10 +380,7 @@ __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
   pdl_wait();
-  auto fail = [&] {
-    atomicExch(a.error_flag, 1);
-    atomicExch(&s_failed, 1);
-  };
+  auto fail = [&] { give_up(a.error_flag, &s_failed); };
 
   if (tid == kPjWarps * 32) {
     // ---- copies, running on from tile to tile
@@ -384,6 +405,7 @@ __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_
         }
       }
     }
+    if (!copies_landed(full, s, round)) fail();
   } else if (tid == (kPjWarps + 1) * 32) {
     // ---- MMAs
     int s = 0, round = 0, n = 0;
@@ -395,7 +417,7 @@ __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       for (int ks = 0; ks < a.k_steps && ok; ks++) {
-        ok = mbar_wait(smem_u32(full + s), round & 1);
+        ok = mbar_wait(smem_u32(full + s), round & 1, kStageTries);
         if (!ok) {
           fail();
           break;
@@ -452,7 +474,8 @@ __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_
       }
       const bool arrived = mbar_wait(smem_u32(accum), n & 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (!__all_sync(~0u, arrived)) {
+      // the MMAs' thread lets the accumulators go on failure too: they are no result then
+      if (!__all_sync(~0u, arrived && !*(volatile int *)&s_failed)) {
         fail();
         continue;
       }
