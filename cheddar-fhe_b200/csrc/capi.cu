@@ -5,6 +5,7 @@
 
 #include <new>
 
+#include "apart.h"
 #include "context.h"
 #include "host_math.h"
 #include "kernels.h"
@@ -103,6 +104,7 @@ static bool all_there(T *const *p, size_t n, bool aligned) {
     if (!p[i] || (aligned && (uintptr_t)p[i] % 16)) return false;
   return true;
 }
+static size_t poly_bytes(int n_limbs) { return (size_t)n_limbs * kN * sizeof(uint32_t); }
 static int check_limbs(const Context &c, const int *gidx, int n_limbs) {
   if (!gidx) return fail("null argument");
   if (n_limbs < 1 || n_limbs > kMaxLimbs) return fail("between one and 64 limbs are expected");
@@ -855,6 +857,13 @@ int cfhe_ctpt_project(cfhe_context *h, uint32_t *const *yb, uint32_t *const *ya,
     if (res_scale && !rb) return fail("projection: a residual scale without a residual");
     for (int j = 0; rb && j < n_out; j++)
       if (!rb[j] != !ra[j]) return fail("projection: a residual needs both polynomials");
+    Outputs outputs(poly_bytes(n_limbs));
+    outputs.add(yb, n_out);
+    outputs.add(ya, n_out);
+    if (!outputs.apart() || outputs.meet(xb, n_in) || outputs.meet(xa, n_in) || (rb && outputs.meet(rb, n_out, yb)) ||
+        (ra && outputs.meet(ra, n_out, ya)) ||
+        outputs.meet(packed, n_limbs * gemm_packed_weight_bytes(n_in, n_out)))
+      return fail("projection: an output overlaps another operand");
     const uint32_t *const *x[2] = {xb, xa}, *const *res[2] = {rb, ra};
     uint32_t *const *y[2] = {yb, ya};
     TableBlob blob;
@@ -903,6 +912,11 @@ static int rotary(Context &c, uint32_t *const *y, const uint32_t *const *x, int 
   const size_t dim = 2 * (size_t)n_pairs, polys = n_rows * dim;
   if (!all_there(x, polys, true) || !all_there(y, polys, true))
     return fail("rotary positions: an operand is null or not on a 16-byte boundary");
+  Outputs outputs(poly_bytes(n_limbs));
+  outputs.add(y, polys);
+  if (!outputs.apart() || outputs.meet(x, polys, y) ||
+      (cos && (outputs.meet(cos, n_pairs) || outputs.meet(sin, n_pairs))))
+    return fail("rotary positions: an output overlaps another operand");
   std::vector<RotarySlot> slots((size_t)n_rows * n_pairs);
   for (size_t r = 0, s = 0; r < (size_t)n_rows; r++)
     for (size_t i = 0; i < (size_t)n_pairs; i++, s++) {
@@ -949,6 +963,11 @@ int cfhe_ctct_gemm(cfhe_context *h, uint32_t *const *d0, uint32_t *const *d1, ui
         !all_there(d0, mn, true) || !all_there(d1, mn, true) || !all_there(d2, mn, true) ||
         (decay_pt && !all_there(decay_pt, mn, true)))
       return fail("ct-ct GEMM: an operand is null or not on a 16-byte boundary");
+    Outputs outputs(poly_bytes(n_limbs));
+    for (uint32_t *const *d : {d0, d1, d2}) outputs.add(d, mn);
+    if (!outputs.apart() || outputs.meet(lb, mk) || outputs.meet(la, mk) || outputs.meet(rb, kn) ||
+        outputs.meet(ra, kn) || (decay_pt && outputs.meet(decay_pt, mn)))
+      return fail("ct-ct GEMM: an output overlaps another operand");
     // the product of the transposes where there are more rows than columns
     const bool turned = m > n;
     CtctArgs a;

@@ -267,7 +267,8 @@ CFHE_API int cfhe_rotary_token(cfhe_context *ctx, uint32_t *const *y, const uint
  * operands; outputs overlap nothing; polynomials on 16-byte boundaries. Same
  * words as cfhe_tensor_accum per result, then cfhe_binary / cfhe_const_op
  * (multiply) on its three parts.
- * The four calls above read their HOST tables before they return and may be captured
+ * The four calls above refuse an output that overlaps another one or an operand (apart
+ * from what is said above), read their HOST tables before they return and may be captured
  * into a graph; a captured projection or product keeps device memory of its own for
  * tables and temporaries until the context is destroyed, which has to outlive the
  * graph. */
