@@ -320,11 +320,28 @@ static int get_cts(PyObject *o, int lead, int parts, int kind, const ct_shape *w
   return 0;
 }
 
-/* host words; None: none. Any other count than `count` is an error. */
-static int get_words(PyObject *o, long long count, int_list *l) {
+/* host words [d0][d1][d2]; None: none. Any other number of them is an error, and so is
+ * an array of two dimensions or more (those of size 1 do not count) that are not these:
+ * it holds the words in another order. */
+static int get_words(PyObject *o, long long d0, long long d1, long long d2, int_list *l) {
   if (get_constants(o, l)) return -1;
-  if (o != Py_None && l->b.len != 4 * count) {
+  if (o == Py_None) return 0;
+  const long long want[3] = {d0, d1, d2};
+  if (l->b.len != 4 * d0 * d1 * d2) {
     PyErr_SetString(PyExc_ValueError, "wrong number of constants");
+    free_ints(l);
+    return -1;
+  }
+  int dims = 0, same = 1, w = 0;
+  for (int i = 0; i < l->b.ndim; i++) {
+    if (l->b.shape[i] == 1) continue;
+    dims++;
+    while (w < 3 && want[w] == 1) w++;
+    same &= w < 3 && l->b.shape[i] == want[w];
+    w++;
+  }
+  if (dims > 1 && !same) {
+    PyErr_SetString(PyExc_ValueError, "constants in another order than the call's");
     free_ints(l);
     return -1;
   }
@@ -760,7 +777,7 @@ static PyObject *py_ctpt_project(PyObject *self, PyObject *const *a, Py_ssize_t 
       goto done;
     }
   }
-  if (get_words(a[6], want.limbs * y.rows, &bias) || get_words(a[8], want.limbs, &scale)) goto done;
+  if (get_words(a[6], want.limbs, y.rows, 1, &bias) || get_words(a[8], want.limbs, 1, 1, &scale)) goto done;
   ENTER(cfhe_ctpt_project(HANDLE(a[0]), (u32 *const *)y.p, (u32 *const *)y.p + y.rows, (const u32 *const *)x.p,
                           (const u32 *const *)x.p + x.rows, w, (int)x.rows, (int)y.rows, bias.p,
                           (const u32 *const *)r.p, r.p ? (const u32 *const *)r.p + r.rows : NULL, scale.p, g.p, g.n));
@@ -799,7 +816,7 @@ static PyObject *py_rotary(PyObject *self, PyObject *const *a, Py_ssize_t n) {
   u32 *const *yp = (u32 *const *)y.p;
   const u32 *const *xp = (const u32 *const *)x.p;
   if (PyObject_CheckBuffer(a[4])) {
-    if (get_words(a[4], pairs * want.limbs, &cw) || get_words(a[5], pairs * want.limbs, &sw)) goto done;
+    if (get_words(a[4], pairs, want.limbs, 1, &cw) || get_words(a[5], pairs, want.limbs, 1, &sw)) goto done;
     ENTER(cfhe_rotary_token(HANDLE(a[0]), yp, xp, (int)(2 * x.rows), (int)pairs, halves != 0, cw.p, sw.p, g.p, g.n));
   } else {
     if (get_cts(a[4], 1, 0, INPUT, &want, &c) || get_cts(a[5], 1, 0, INPUT, &want, &s)) goto done;
@@ -845,7 +862,7 @@ static PyObject *py_ctct_gemm(PyObject *self, PyObject *const *a, Py_ssize_t n) 
   const Py_ssize_t mn = d.rows * d.cols, mk = l.rows * l.cols, kn = r.rows * r.cols;
   if (a[6] != Py_None) {
     if (PyObject_CheckBuffer(a[6])) {
-      if (get_words(a[6], mn * want.limbs, &ww)) goto done;
+      if (get_words(a[6], d.rows, d.cols, want.limbs, &ww)) goto done;
     } else {
       if (get_cts(a[6], 2, 0, INPUT, &want, &w)) goto done;
       if (w.rows != d.rows || w.cols != d.cols) {
