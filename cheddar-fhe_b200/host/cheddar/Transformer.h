@@ -91,6 +91,9 @@ struct TransformerConfig {
   bool rotary_halves = false;
   bool pair_boot = true;  // bootstrap two real ciphertexts as one complex one
   int workers = 4;        // host threads (and streams) of the per-ciphertext stages
+  // unrelinearised products of ciphertexts (three polynomials each) that attention
+  // holds at a time, whatever the sequence: 128 take 1.2 GB on 12 limbs
+  int products = 128;
   static TransformerConfig BertBase() { return TransformerConfig{}; }
   static TransformerConfig Small() {
     TransformerConfig c;
@@ -189,6 +192,25 @@ inline std::vector<std::vector<double>> RotaryAngles(const std::vector<int> &pai
   AssertTrue((int)angles.size() <= pairs, "Rotary: the axes have more pairs than a head");
   angles.resize(pairs, std::vector<double>(tokens, 0.0));
   return angles;
+}
+
+// The m x n results of a product of ciphertexts in blocks of at most `results`, one row
+// of blocks after the other. Blocks span the shorter side where that fits, so that the
+// operand of the longer side is read once.
+struct ProductBlock {
+  int i0, i1, j0, j1;
+};
+inline std::vector<ProductBlock> ProductBlocks(int m, int n, int results) {
+  AssertTrue(m > 0 && n > 0 && results > 0, "ProductBlocks: positive sizes are needed");
+  const int rows_at_most = m <= n ? Min(m, results) : Min(m, Max(1, results / Min(n, results)));
+  const int cols_at_most = Min(n, Max(1, results / rows_at_most));
+  const int rows = (m + rows_at_most - 1) / rows_at_most, cols = (n + cols_at_most - 1) / cols_at_most;
+  std::vector<ProductBlock> blocks;
+  for (int r = 0; r < rows; r++)
+    for (int c = 0; c < cols; c++)
+      blocks.push_back({(int)((long long)m * r / rows), (int)((long long)m * (r + 1) / rows),
+                        (int)((long long)n * c / cols), (int)((long long)n * (c + 1) / cols)});
+  return blocks;
 }
 
 // A plaintext matrix encoded on the limbs of one level and packed for the
@@ -924,19 +946,15 @@ class EncryptedTransformerLayer {
         const int g = 1 + i / D, d = i % D;
         RotateTokens(c, qg[g][d], Q(d), -g * nb, evk);
       });
-      std::vector<Ct> acc;  // of the main context, freed after the loop
-      {
-        std::vector<const Ct *> left, right;
-        for (int g = 0; g < ng; g++)
-          for (int d = 0; d < D; d++) left.push_back(g ? &qg[g][d] : &Q(d));
-        for (int d = 0; d < D; d++)
-          for (int b = 0; b < nb; b++) right.push_back(&kb[d][b]);
-        ctx_->MultMatrixUnsafe(acc, left, right, ng, D, nb);
-      }
-      ParallelFor(T, [&](const Cx &c, int r) {
-        const int g = r / nb;
+      std::vector<const Ct *> left, right;
+      for (int g = 0; g < ng; g++)
+        for (int d = 0; d < D; d++) left.push_back(g ? &qg[g][d] : &Q(d));
+      for (int d = 0; d < D; d++)
+        for (int b = 0; b < nb; b++) right.push_back(&kb[d][b]);
+      Products(left, right, ng, D, nb, {}, [&](const Cx &c, int g, int b, const Ct &product) {
+        const int r = g * nb + b;
         Ct u;
-        c->RelinearizeRescale(u, acc[r], mult);
+        c->RelinearizeRescale(u, product, mult);
         if (g) {
           Ct rot;
           RotateTokens(c, rot, u, g * nb, evk);
@@ -978,29 +996,58 @@ class EncryptedTransformerLayer {
     const int D = cfg_.head_dim, nb = cfg_.baby, ng = cfg_.seq_len / nb;
     const Evk &mult = evk.GetMultiplicationKey();
     using Cx = ConstContextPtr<word>;
-    std::vector<Ct> acc;  // of the main context, freed after the loop
-    {
-      std::vector<const Ct *> right;
-      for (int b = 0; b < nb; b++)
-        for (int d = 0; d < D; d++) right.push_back(&vb[d][b]);
-      ctx_->MultMatrixUnsafe(acc, weights, right, ng, nb, D);
-    }
-    std::vector<std::vector<Ct>> part(ng);
+    std::vector<const Ct *> right;
+    for (int b = 0; b < nb; b++)
+      for (int d = 0; d < D; d++) right.push_back(&vb[d][b]);
+    std::vector<std::vector<Ct>> part(ng);  // of the block at hand
     for (int g = 0; g < ng; g++) part[g].resize(D);
-    ParallelFor(ng * D, [&](const Cx &c, int i) {
-      const int g = i / D, d = i % D;
+    Products(weights, right, ng, nb, D, {}, [&](const Cx &c, int g, int d, const Ct &product) {
       Ct t;
-      c->RelinearizeRescale(t, acc[i], mult);
+      c->RelinearizeRescale(t, product, mult);
       if (g)
         RotateTokens(c, part[g][d], t, g * nb, evk);
       else
         part[0][d] = std::move(t);
+    }, [&](const ProductBlock &block) {
+      ParallelFor(block.j1 - block.j0, [&](const Cx &c, int i) {
+        const int d = block.j0 + i;
+        Ct &dst = o[h * D + d];
+        for (int g = block.i0; g < block.i1; g++)
+          if (g)
+            c->Add(dst, dst, part[g][d]);  // in place: it keeps its buffers
+          else
+            c->Copy(dst, part[0][d]);
+      });
+      for (int g = block.i0; g < block.i1; g++)
+        for (int d = block.j0; d < block.j1; d++) part[g][d] = Ct();
     });
-    ParallelFor(D, [&](const Cx &c, int d) {
-      Ct &dst = o[h * D + d];
-      c->Copy(dst, part[0][d]);
-      for (int g = 1; g < ng; g++) c->Add(dst, dst, part[g][d]);
-    });
+  }
+
+  // use(context, i, j, product) of every product (decay[i n + j] (*)) sum_t left[i k + t]
+  // right[t n + j] of an m x k and a k x n matrix, shared out over the worker threads;
+  // cfg_.products of them are held at a time, in blocks of whole columns where those
+  // fit, each block followed by then(block).
+  template <typename Use>
+  void Products(const std::vector<const Ct *> &left, const std::vector<const Ct *> &right, int m, int k, int n,
+                const std::vector<const Plaintext<word> *> &decay, Use &&use,
+                const std::function<void(const ProductBlock &)> &then = {}) {
+    for (const ProductBlock &x : ProductBlocks(m, n, cfg_.products)) {
+      const int rows = x.i1 - x.i0, cols = x.j1 - x.j0;
+      std::vector<const Ct *> some;
+      for (int t = 0; t < k; t++)
+        for (int j = x.j0; j < x.j1; j++) some.push_back(right[(size_t)t * n + j]);
+      std::vector<const Plaintext<word> *> weights;
+      for (int i = x.i0; !decay.empty() && i < x.i1; i++)
+        for (int j = x.j0; j < x.j1; j++) weights.push_back(decay[(size_t)i * n + j]);
+      std::vector<Ct> acc;  // of the main context, freed after the loop
+      ctx_->MultMatrixUnsafe(acc, {left.begin() + (size_t)x.i0 * k, left.begin() + (size_t)x.i1 * k}, some, rows, k,
+                             cols, weights);
+      ParallelFor(rows * cols, [&](const ConstContextPtr<word> &c, int i) {
+        use(c, x.i0 + i / cols, x.j0 + i % cols, acc[i]);
+      });
+      acc.clear();
+      if (then) then(x);
+    }
   }
 
   // Queries and keys of heads [head0, head1) turned by their tokens' positions, one
@@ -1072,12 +1119,10 @@ class EncryptedTransformerLayer {
                            ctx_->param_.GetRescalePrimeProd(l) / (left[0]->GetScale() * right[0]->GetScale());
       std::vector<const Plaintext<word> *> decay;
       for (int r = 0; r < T; r++) decay.push_back(&DecayMask(cfg_.decay[h], r, l, scale));
-      std::vector<Ct> acc;  // of the main context, freed after the loop
-      ctx_->MultMatrixUnsafe(acc, left, right, ng, D, nb, decay);
-      ParallelFor(T, [&](const Cx &c, int r) {
+      Products(left, right, ng, D, nb, decay, [&](const Cx &c, int g, int b, const Ct &product) {
         Ct once;
-        c->RelinearizeRescale(once, acc[r], mult);
-        c->Rescale(weights[r], once);
+        c->RelinearizeRescale(once, product, mult);
+        c->Rescale(weights[g * nb + b], once);
       });
     }
     const int lw = Level(weights[0]);
