@@ -11,7 +11,7 @@ CPP = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("mode", ["blocks softmax", "blocks linear"])
+@pytest.mark.parametrize("mode", ["blocks softmax", "blocks linear", "ranks softmax", "ranks linear", "rotary"])
 def test_layer_forms(pkg, mode):
     if not os.path.exists(pkg.LIB_PATH):
         pkg.build()
