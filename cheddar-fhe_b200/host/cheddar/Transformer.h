@@ -663,6 +663,12 @@ class EncryptedTransformerLayer {
   double PackSeconds() const { return pack_s_; }  // encoding and packing the weights (first Forward only)
   double GemmInt8Macs() const { return gemm_macs_; }
   int Bootstraps() const { return boots_; }
+  // weights of linear attention and of rotary positions that stay on the device
+  int KeptPlaintexts() const {
+    size_t n = cos_.size() + sin_.size();
+    for (const auto &d : decays_) n += d.second.size();
+    return (int)n;
+  }
 
  private:
   int Level(const Ct &c) const { return ctx_->param_.NPToLevel(c.GetNP()); }
@@ -1117,9 +1123,7 @@ class EncryptedTransformerLayer {
       const int l = Level(*left[0]);
       const double scale = Canon(l - 2) * ctx_->param_.GetRescalePrimeProd(l - 1) *
                            ctx_->param_.GetRescalePrimeProd(l) / (left[0]->GetScale() * right[0]->GetScale());
-      std::vector<const Plaintext<word> *> decay;
-      for (int r = 0; r < T; r++) decay.push_back(&DecayMask(cfg_.decay[h], r, l, scale));
-      Products(left, right, ng, D, nb, decay, [&](const Cx &c, int g, int b, const Ct &product) {
+      Products(left, right, ng, D, nb, DecayMasks(cfg_.decay[h], l, scale), [&](const Cx &c, int g, int b, const Ct &product) {
         Ct once;
         c->RelinearizeRescale(once, product, mult);
         c->Rescale(weights[g * nb + b], once);
@@ -1135,24 +1139,35 @@ class EncryptedTransformerLayer {
     WeightedValues(h, Pointers(weights), vb, o, evk);
   }
 
-  // decay^(t - u) at slot (t + g nb) B + b for the tokens t that see token u = t + r
-  // (mod T), 0 for the others
-  const Plaintext<word> &DecayMask(double decay, int r, int level, double scale) {
-    const auto key = std::make_tuple(decay, r, level, scale);
-    auto it = decays_.find(key);
-    if (it == decays_.end()) {
-      const int T = cfg_.seq_len, turned = r / cfg_.baby * cfg_.baby;
-      std::vector<Complex> msg(slots_);
-      for (int t = 0; t < T; t++) {
-        const int u = (t + r) % T;
-        const double w = u <= t ? std::pow(decay, t - u) : 0.0;
-        for (int b = 0; b < lane_; b++) msg[(size_t)((t + turned) % T) * lane_ + b] = Complex(w, 0.0);
-      }
-      Plaintext<word> pt;
-      ctx_->encoder().Encode(pt, level, scale, msg, 0);
-      it = decays_.emplace(key, std::move(pt)).first;
+  // The weights of the scores of heads with this decay: for offset r, decay^(t - u) at
+  // slot (t + g nb) B + b for the tokens t that see token u = t + r (mod T), 0 for the
+  // others. Encoded by all host threads when a decay is first met, and kept for the
+  // calls that follow: seq_len plaintexts a decay, on one level and scale at a time.
+  std::vector<const Plaintext<word> *> DecayMasks(double decay, int level, double scale) {
+    if (!decays_.empty()) {
+      const Plaintext<word> &kept = decays_.begin()->second[0];
+      if (ctx_->param_.NPToLevel(kept.GetNP()) != level || std::abs(kept.GetScale() - scale) > 1e-12 * scale)
+        decays_.clear();
     }
-    return it->second;
+    std::vector<Plaintext<word>> &masks = decays_[decay];
+    if (masks.empty()) {
+      const int T = cfg_.seq_len;
+      std::vector<Plaintext<word>> fresh(T);
+      ParallelFor(T, [&](const ConstContextPtr<word> &c, int r) {
+        const int turned = r / cfg_.baby * cfg_.baby;
+        std::vector<Complex> msg(slots_);
+        for (int t = 0; t < T; t++) {
+          const int u = (t + r) % T;
+          const double w = u <= t ? std::pow(decay, t - u) : 0.0;
+          for (int b = 0; b < lane_; b++) msg[(size_t)((t + turned) % T) * lane_ + b] = Complex(w, 0.0);
+        }
+        c->encoder().Encode(fresh[r], level, scale, msg, 0);
+      });
+      masks = std::move(fresh);
+    }
+    std::vector<const Plaintext<word> *> p;
+    for (const auto &m : masks) p.push_back(&m);
+    return p;
   }
 
   // z[j] = gamma_j y[j] / sqrt(var + eps) + beta_j / act_div for centred y
@@ -1295,9 +1310,9 @@ class EncryptedTransformerLayer {
   std::unique_ptr<PlainMatrix<word>> m_qkv_, m_wo_, m_w1_, m_w2_, m_res_;
   Probe probe_;
   std::map<std::tuple<int, double, double>, Plaintext<word>> masks_;
-  std::map<std::tuple<double, int, int, double>, Plaintext<word>> decays_;  // decay, offset, level, scale
-  std::vector<std::vector<double>> angles_;                                 // of the rotary positions, [pair][token]
-  std::vector<Plaintext<word>> cos_, sin_;                                  // encoded at the level they are used on
+  std::map<double, std::vector<Plaintext<word>>> decays_;  // [offset], of every decay met
+  std::vector<std::vector<double>> angles_;                // of the rotary positions, [pair][token]
+  std::vector<Plaintext<word>> cos_, sin_;                 // encoded at the level they are used on
   std::vector<double> mask_signs_;
   std::vector<std::pair<std::string, double>> stage_s_;
   std::chrono::steady_clock::time_point last_;

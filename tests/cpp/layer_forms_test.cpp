@@ -4,6 +4,7 @@
 //
 //   layer_forms_test <parameter.json> blocks softmax|linear  attention's products in blocks of any size
 //   layer_forms_test <parameter.json> ranks softmax|linear   two ranks against one
+//   layer_forms_test <parameter.json> again                  linear attention's kept weights, called again
 //   layer_forms_test <parameter.json> rotary                 softmax attention with rotary positions
 //
 // The two ranks are threads of this process, each with contexts of its own, on one GPU.
@@ -181,6 +182,24 @@ static void Ranks(Setup &s) {
   }
 }
 
+// Inputs whose scale differs in the last place (what a stack of layers hands on) find
+// the kept weights, and the same inputs leave the same words.
+static void Again(Setup &s) {
+  EncryptedTransformerLayer<word> layer(s.ctx, s.cfg, s.w);
+  std::vector<Ciphertext<word>> out;
+  layer.Forward(out, s.in, s.ui->GetEvkMap());
+  const Words first = WordsOf(out);
+  const int kept = layer.KeptPlaintexts();
+  AssertTrue(kept == 2 * s.cfg.seq_len + s.cfg.head_dim, "FAIL: weights of two decays, and a cosine and sine per pair");
+  const double scale = s.in[0].GetScale();
+  for (int ulps = -2; ulps <= 2; ulps++) {
+    for (auto &c : s.in) c.SetScale(scale * (1.0 + ulps * std::ldexp(1.0, -52)));
+    layer.Forward(out, s.in, s.ui->GetEvkMap());
+    AssertTrue(layer.KeptPlaintexts() == kept, "FAIL: " + std::to_string(layer.KeptPlaintexts()) + " plaintexts are kept");
+    if (ulps == 0) AssertTrue(WordsOf(out) == first, "FAIL: other words from the same inputs");
+  }
+}
+
 // The textbook layer with rotary positions before softmax; `zero` leaves them out
 static std::vector<double> Plain(const std::vector<double> &x, const plain_transformer::Spec &s,
                                  const plain_transformer::Weights &w, const plain_decoder::Positions &p, bool zero,
@@ -278,16 +297,18 @@ static void Rotary(Setup &s) {
 
 int main(int argc, char **argv) {
   if (argc < 3) {
-    std::cerr << "usage: layer_forms_test <parameter.json> blocks|ranks softmax|linear | rotary\n";
+    std::cerr << "usage: layer_forms_test <parameter.json> blocks|ranks softmax|linear | again | rotary\n";
     return 2;
   }
   const std::string mode = argv[2];
-  const bool linear = argc > 3 && !strcmp(argv[3], "linear");
+  const bool linear = mode == "again" || (argc > 3 && !strcmp(argv[3], "linear"));
   Setup s(argv[1], linear, linear || mode == "rotary");
   if (mode == "blocks")
     Blocks(s);
   else if (mode == "ranks")
     Ranks(s);
+  else if (mode == "again")
+    Again(s);
   else
     Rotary(s);
   std::cout << "PASS\n";

@@ -1,5 +1,5 @@
 """Forms of the encrypted transformer layer that have to leave the same words: attention's
-products in blocks of any size, one rank or two, softmax or linear attention; and softmax
+products in blocks of any size, one rank or two, softmax or linear attention, called again; and softmax
 attention with rotary positions against float64 (tests/cpp/layer_forms_test.cpp). Parity
 unpinned by the reference, which has no transformer code."""
 import os
@@ -11,7 +11,7 @@ CPP = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("mode", ["blocks softmax", "blocks linear", "ranks softmax", "ranks linear", "rotary"])
+@pytest.mark.parametrize("mode", ["blocks softmax", "blocks linear", "ranks softmax", "ranks linear", "again", "rotary"])
 def test_layer_forms(pkg, mode):
     if not os.path.exists(pkg.LIB_PATH):
         pkg.build()
