@@ -858,8 +858,7 @@ int cfhe_ctpt_project(cfhe_context *h, uint32_t *const *yb, uint32_t *const *ya,
     for (int j = 0; rb && j < n_out; j++)
       if (!rb[j] != !ra[j]) return fail("projection: a residual needs both polynomials");
     Outputs outputs(poly_bytes(n_limbs));
-    outputs.add(yb, n_out);
-    outputs.add(ya, n_out);
+    outputs.add({yb, ya}, n_out);
     if (!outputs.apart() || outputs.meet(xb, n_in) || outputs.meet(xa, n_in) || (rb && outputs.meet(rb, n_out, yb)) ||
         (ra && outputs.meet(ra, n_out, ya)) ||
         outputs.meet(packed, n_limbs * gemm_packed_weight_bytes(n_in, n_out)))
@@ -913,7 +912,10 @@ static int rotary(Context &c, uint32_t *const *y, const uint32_t *const *x, int 
   if (!all_there(x, polys, true) || !all_there(y, polys, true))
     return fail("rotary positions: an operand is null or not on a 16-byte boundary");
   Outputs outputs(poly_bytes(n_limbs));
-  outputs.add(y, polys);
+  if (n_rows % 2)
+    outputs.add({y}, polys);
+  else  // the rows of b polynomials, then those of a
+    outputs.add({y, y + polys / 2}, polys / 2);
   if (!outputs.apart() || outputs.meet(x, polys, y) ||
       (cos && (outputs.meet(cos, n_pairs) || outputs.meet(sin, n_pairs))))
     return fail("rotary positions: an output overlaps another operand");
@@ -964,7 +966,7 @@ int cfhe_ctct_gemm(cfhe_context *h, uint32_t *const *d0, uint32_t *const *d1, ui
         (decay_pt && !all_there(decay_pt, mn, true)))
       return fail("ct-ct GEMM: an operand is null or not on a 16-byte boundary");
     Outputs outputs(poly_bytes(n_limbs));
-    for (uint32_t *const *d : {d0, d1, d2}) outputs.add(d, mn);
+    outputs.add({d0, d1, d2}, mn);
     if (!outputs.apart() || outputs.meet(lb, mk) || outputs.meet(la, mk) || outputs.meet(rb, kn) ||
         outputs.meet(ra, kn) || (decay_pt && outputs.meet(decay_pt, mn)))
       return fail("ct-ct GEMM: an output overlaps another operand");

@@ -14,8 +14,8 @@ typedef const char *const *P;
 // 1: refused
 extern "C" int refused(size_t bytes, P y, int ny, P x, int nx, P own, size_t w, size_t w_bytes) {
   cfhe::Outputs o(bytes);
-  o.add(y, ny / 2);
-  o.add(y + ny / 2, ny - ny / 2);
+  o.add({y, y + ny / 2}, ny / 2);
+  o.add({y + ny / 2 * 2}, ny % 2);
   return !o.apart() || o.meet(x, nx, own) || (w_bytes && o.meet((const void *)w, w_bytes));
 }
 """
