@@ -15,19 +15,26 @@
 // run ahead of the products over tile ends, and the pointers ahead of the copies.
 //
 // C is 64 or more: every row is another page, and an SM gets to a page that it did
-// not visit shortly before about every eight clocks, so rows of 64, 128 and 256
-// bytes come at 2.4, 4.5 and 6.2 TB/s at most (8.9 from L2).
+// not visit shortly before about every eight clocks, so rows of 64 and 128 bytes come
+// at 2.5 and 4.5 TB/s at most, of 256 bytes at 6.4 to 7.0 (8.9 from L2).
 //
-// m <= 2: bound by reading R, whose words enter one or two results. m >= 3: bound by
-// the multipliers. A 32 x 32 + 64-bit multiply-add is three instructions here, and
-// 64-bit sums of products have to be folded; so a sum T of products is kept twice, as
+// m <= 2: bound by reading R, whose words enter one or two results, where there are
+// terms enough: 0.73 to 0.83 of the copy rate for one row and 60 terms or more, 0.65
+// for 2 x 64 x 64. Where a block has few stages, by the latency of the first and of the
+// stores: 0.45 for 2 x 9 x 13, 0.35 for 1 x 5 x 9.
+//
+// m >= 3: bound by the multipliers. A 32 x 32 + 64-bit multiply-add is three instructions
+// here, and 64-bit sums of products have to be folded; so a sum T of products is kept twice, as
 // its low 32 bits (32-bit multiply-adds) and as a double (rounded), one instruction
 // each:  T mod q = T - q round(T / q), which only needs the low bits of T and a T / q
 // that is off by less than a quarter. Three products a term: b a' + a b' comes from the
-// product of the sums. The two kinds of multiply-add hardly overlap (24 of each for
-// four warps: 270 and 387 clocks alone, 590 to 710 together), which is 3.8 of the 5.3
-// ms of 8 x 64 x 16 on 14 limbs. With 64-bit sums it took 6.6 ms, with four products a
-// term and each result's weight fetched on its own 6.0; bytes on the tensor cores
+// product of the sums. The two kinds of multiply-add hold each other up. 24 of each for
+// four warps, operands in registers: the 32-bit ones take 270 clocks, the double ones
+// 387 (221 to 283 if no operand were subnormal, as those of tiny() are), both 712 (644
+// to 661), more than one after the other; 592 with operands from shared memory, which
+// is 3.8 of the 5.4 ms of 8 x 64 x 16 on 14 limbs. No pipe is full meanwhile and the
+// stall is in dispatch; what causes it is not known. With 64-bit sums it took 6.6 ms,
+// with four products a term and each result's weight fetched on its own 6.0; bytes on the tensor cores
 // (tcgen05.mma wants 64 rows, a position has 2 n; mma.sync with operands split into byte
 // planes, whose seven 32-bit sums a result only fit tensor memory and leave a tile of
 // 4 x 8) 6.1; copies of whole rows that the warps wait for one by one, so that they may

@@ -337,10 +337,10 @@ __global__ void __launch_bounds__(kGmThreads, 2) gemm_tc_kernel(const __grid_con
 // entries); copies and, once the epilogue has fetched its accumulators, MMAs of the
 // next tile go on under the epilogue of the last. Eight epilogue warps: with a
 // residual a word takes some 35 instructions, so few inputs (32: two K steps a tile)
-// leave the epilogue the longer part. Against a CTA a tile: 32 x 64 on 3 limbs
-// 95 -> 82 us, 130 x 77 with a residual on 9 limbs 770 -> 690 us; 768 x 768 on 11
-// limbs takes 12.2 to 13.1 ms either way, at the power limit. (With the failure flag
-// read at the top of a tile and larger groups 76 and 654 us.)
+// leave the epilogue the longer part. CTAs that stay took 14 % less than a CTA a tile
+// for 32 x 64 on 3 limbs and 10 % less for 130 x 77 with a residual on 9 limbs (77 and
+// 653 us now); 768 x 768 on 11 limbs takes 12.2 to 13.1 ms either way, at the power
+// limit.
 constexpr int kPjWarps = 8, kPjThreads = 32 * (kPjWarps + 2), kPjOuts = kGmOutTile / 2;
 
 __global__ void __launch_bounds__(kPjThreads, 2) project_tc_kernel(const __grid_constant__ GemmArgs a,
@@ -636,9 +636,9 @@ int launch_ctpt_gemm(const Context &c, uint32_t *const *y, const uint32_t *const
 //
 // From three output tiles on an entry's activations are packed inside the products
 // of the entry before (two buffers); with fewer, entries go in groups of up to 96 MiB
-// of packed activations (they and a group's results stay in L2), two launches a group (packing inside the products was slower:
-// 130 x 77 on 9 limbs 1.00 instead of 0.78 ms; 0.70 ms in groups of one, 0.67 of two, 0.66 of
-// four).
+// of packed activations (they and a group's results stay in L2), two launches a group.
+// For 130 x 77 on 9 limbs packing inside the products took 28 % longer; groups of one,
+// two and four entries took 0.70, 0.67 and 0.66 ms.
 int project_buffers(int n_in, int n_out, int n_limbs) {
   if (gemm_packs_ahead(n_out, 2 * n_limbs)) return 2;
   const size_t fit = ((size_t)96 << 20) / gemm_scratch_bytes(n_in);
