@@ -310,7 +310,9 @@ class Engine:
         polynomials (cfhe_ctpt_project). y, residual: [n_out, 2, limbs, N], x: [n_in, 2,
         limbs, N]; a list of residuals may hold None. bias: uint32 [limbs][n_out], res_scale:
         uint32 [limbs] (None: 1), both M-form on the host. residual may be y."""
-        if packed.numel() < self.gemm_weight_bytes(len(x), len(y), len(gidx)):
+        if not packed.is_contiguous():
+            raise ValueError("the packed weights have to lie one after the other")
+        if packed.numel() * packed.element_size() < self.gemm_weight_bytes(len(x), len(y), len(gidx)):
             raise ValueError("the packed weights are those of a smaller matrix")
         self._check(self.K.ctpt_project(self.hp, self.device, y, x, packed, gidx, bias, residual, res_scale))
 
