@@ -1031,8 +1031,8 @@ class EncryptedTransformerLayer {
 
   // use(context, i, j, product) of every product (decay[i n + j] (*)) sum_t left[i k + t]
   // right[t n + j] of an m x k and a k x n matrix, shared out over the worker threads;
-  // cfg_.products of them are held at a time, in blocks of whole columns where those
-  // fit, each block followed by then(block).
+  // at most cfg_.products of them are held at a time (ProductBlocks), each block
+  // followed by then(block).
   template <typename Use>
   void Products(const std::vector<const Ct *> &left, const std::vector<const Ct *> &right, int m, int k, int n,
                 const std::vector<const Plaintext<word> *> &decay, Use &&use,
@@ -1123,7 +1123,8 @@ class EncryptedTransformerLayer {
       const int l = Level(*left[0]);
       const double scale = Canon(l - 2) * ctx_->param_.GetRescalePrimeProd(l - 1) *
                            ctx_->param_.GetRescalePrimeProd(l) / (left[0]->GetScale() * right[0]->GetScale());
-      Products(left, right, ng, D, nb, DecayMasks(cfg_.decay[h], l, scale), [&](const Cx &c, int g, int b, const Ct &product) {
+      const auto masks = DecayMasks(cfg_.decay[h], l, scale);
+      Products(left, right, ng, D, nb, masks, [&](const Cx &c, int g, int b, const Ct &product) {
         Ct once;
         c->RelinearizeRescale(once, product, mult);
         c->Rescale(weights[g * nb + b], once);
